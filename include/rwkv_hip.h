@@ -428,6 +428,73 @@ int rwkv_model_decode_sample(rwkv_model *m, rwkv_stream_t stream,
 int rwkv_argmax_f64(rwkv_stream_t stream, const double *logits, int64_t V,
                     int64_t *out_token);
 
+/* ------------------------------------------------------------------------
+ * 5. Operators of a serving step over the rows of many requests.  The
+ *    reference has no counterpart of them; they stand beside the products, the
+ *    recurrence and the sampler above.  Row strides are in elements.
+ * ---------------------------------------------------------------------- */
+
+typedef enum rwkv_type { RWKV_F32 = 0, RWKV_F64 = 1, RWKV_BF16 = 2, RWKV_F16 = 3 } rwkv_type;
+
+/* Low-rank adapters of many requests beside a projection that they share:
+ *   out[t] = base[t] + scale[i] * b[i] (a[i] x[t]),  i = adapter[t],  t < T.
+ * x [T, n_in], base and out [T, n_out] of type `real` (RWKV_F32 or RWKV_F64, which
+ * is also what products and sums are computed in), rows x_stride, base_stride and
+ * out_stride apart; a [N, R, n_in], b [N, n_out, R] of type `low` (RWKV_BF16,
+ * RWKV_F16 or RWKV_F32), R <= 256 (adapters of smaller rank are filled with
+ * zeros); adapter int32 [T]: a row whose number is not in 0..N-1 has none and
+ * gets base[t].  scale float32 [N] or NULL (= 1); base NULL (= 0) or any rows, out
+ * itself among them.  What a row holds (infinities, NaN) reaches no other row.
+ * workspace: rwkv_lora_rows_workspace_bytes bytes, 16-byte aligned. */
+size_t rwkv_lora_rows_workspace_bytes(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real);
+int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R,
+                   int real, const void *x, int64_t x_stride,
+                   int low, const void *a, const void *b,
+                   const int32_t *adapter, const float *scale,
+                   const void *base, int64_t base_stride, void *out, int64_t out_stride,
+                   void *workspace, size_t workspace_bytes);
+
+/* The gated delta rule over B packed sequences, float32 state and sums:
+ *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q
+ * per value head h with the key head h / (Hv / Hk).  q, k [T, Hk, dk], v, o
+ * [T, Hv, dv] of type `type` (RWKV_F32, RWKV_BF16 or RWKV_F16), heads contiguous, rows
+ * q_stride, k_stride, v_stride and Hv * dv apart; g (the logarithm of the decay,
+ * at most 0) and beta float32 [T, Hv]; state float32 [B, Hv, dk, dv], updated in
+ * place.  starts int32 [B + 1] on the device: sequence b is the rows starts[b] ..
+ * starts[b+1] - 1, cut to 0 .. T; NULL: T / B rows each (T a multiple of B).  Rows of
+ * no sequence are left as they were in o, and the state of an empty sequence is.
+ * dk <= 256.  workspace: rwkv_delta_rule_workspace_bytes bytes, 16-byte aligned. */
+size_t rwkv_delta_rule_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv);
+int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,
+                    int type, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                    const void *v, int64_t v_stride, const float *g, const float *beta, float scale,
+                    const int32_t *starts, float *state, void *o,
+                    void *workspace, size_t workspace_bytes);
+
+/* Drafted tokens held against the target's distribution (speculative sampling):
+ * with p_i = softmax(logits[b, i] / temp) and q_i = softmax(draft_logits[b, i] / temp)
+ * draft d_i = drafts[b, i] is accepted while u[b, i] q_i(d_i) < p_i(d_i).  At the first one
+ * refused, i = n, a token is drawn from max(p_n - q_n, 0) (from p_n where that is
+ * nothing), after the last draft from p_n: the lowest index at which the running
+ * weight exceeds u[b, K] times the whole.  greedy: accepted while d_i is the first
+ * maximum of logits[b, i]; the token is that maximum (u, draft_logits, temp unused).
+ *   logits [B, K+1, V], draft_logits [B, K, V] of type `real` (RWKV_F64 or RWKV_F32), all arithmetic
+ * float64; rows of a sequence and sequences the given strides apart; draft_logits
+ * NULL: drafts without a distribution (q_i is 1 at d_i).  drafts int64 [B, K], a
+ * number outside the vocabulary is refused; lengths int32 [B] or NULL: how many of
+ * the K drafts count, cut to 0 .. K; u float32 [B, K+1] in [0, 1).  K <= 64.  A logit that is
+ * -infinity or NaN has no weight, +infinity all of it.
+ *   tokens int64 [B, K+1]: the accepted drafts, the token drawn, then -1 (in the
+ * drawn token's place too, where no logit of the row has weight); accepted int64 [B].
+ * workspace: rwkv_verify_drafts_workspace_bytes bytes, 16-byte aligned. */
+size_t rwkv_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
+int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, int real,
+                       const void *logits, int64_t logits_seq_stride, int64_t logits_row_stride,
+                       const void *draft_logits, int64_t draft_seq_stride, int64_t draft_row_stride,
+                       const int64_t *drafts, const int32_t *lengths, const float *u, double temp, int greedy,
+                       int64_t *tokens, int64_t *accepted,
+                       void *workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

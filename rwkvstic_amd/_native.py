@@ -27,6 +27,8 @@ EXPORTS = (
     "rwkv_sample_token", "rwkv_model_decode_sample",
     "rwkv_gemm8_workspace_bytes", "rwkv_gemm8", "rwkv_gemm8_plan",
     "rwkv_model_batch_workspace_bytes", "rwkv_model_forward_batch",
+    "rwkv_lora_rows_workspace_bytes", "rwkv_lora_rows", "rwkv_delta_rule_workspace_bytes", "rwkv_delta_rule",
+    "rwkv_verify_drafts_workspace_bytes", "rwkv_verify_drafts",
 )
 
 
@@ -128,6 +130,15 @@ def lib() -> C.CDLL:
     L.rwkv_model_batch_workspace_bytes.restype = sz
     L.rwkv_model_batch_workspace_bytes.argtypes = [vp, i64]
     L.rwkv_model_forward_batch.argtypes = [vp, vp, vp, i64, vp, vp, vp, sz]
+    L.rwkv_lora_rows_workspace_bytes.restype = sz
+    L.rwkv_lora_rows_workspace_bytes.argtypes = [i64] * 5 + [ci]
+    L.rwkv_lora_rows.argtypes = [vp] + [i64] * 5 + [ci, vp, i64, ci, vp, vp, vp, vp, vp, i64, vp, i64, vp, sz]
+    L.rwkv_delta_rule_workspace_bytes.restype = sz
+    L.rwkv_delta_rule_workspace_bytes.argtypes = [i64] * 6
+    L.rwkv_delta_rule.argtypes = [vp] + [i64] * 6 + [ci, vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, vp, vp, vp, sz]
+    L.rwkv_verify_drafts_workspace_bytes.restype = sz
+    L.rwkv_verify_drafts_workspace_bytes.argtypes = [i64] * 3
+    L.rwkv_verify_drafts.argtypes = [vp, i64, i64, i64, ci, vp, i64, i64, vp, i64, i64, vp, vp, vp, f64, ci, vp, vp, vp, sz]
     for name in EXPORTS:
         getattr(L, name)          # AttributeError here means header and library disagree
     _lib = L

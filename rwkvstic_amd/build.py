@@ -14,7 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "librwkv_hip.so")
 HOST_LIB = os.path.join(HERE, "_rwkv_torch.so")
-SOURCES = ["rwkv_quant.hip", "rwkv_ops.hip", "rwkv_model.hip", "rwkv_decode.hip", "rwkv_rows.hip", "rwkv_sample.hip"]
+SOURCES = ["rwkv_quant.hip", "rwkv_ops.hip", "rwkv_model.hip", "rwkv_decode.hip", "rwkv_rows.hip", "rwkv_sample.hip",
+           "rwkv_lora.hip", "rwkv_delta.hip", "rwkv_verify.hip"]
 
 FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "-shared",

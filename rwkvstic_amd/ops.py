@@ -364,3 +364,145 @@ def argmax(logits: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Te
     _buffer(out, torch.int64, 1, "out")
     N.check(N.lib().rwkv_argmax_f64(_stream(), logits.data_ptr(), logits.numel(), out.data_ptr()))
     return out
+
+
+# ---------------------------------------------------------------- operators of a serving step over the rows of many requests
+_TYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}         # rwkv_type
+
+
+def _is(t, dtypes, shape, name: str, device=None) -> None:
+    """A CUDA tensor of one of these types and of this shape, on ``device``."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+
+
+def _rows(t: torch.Tensor, name: str) -> int:
+    """The distance of the rows of ``t [T, ...]``, each of them contiguous."""
+    if t.numel() and not t[0].is_contiguous():
+        raise ValueError(f"{name} must have contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else t[0].numel() if t.shape[0] else 0
+
+
+def _apart(t: torch.Tensor, name: str) -> None:
+    """Rows that are written must not share memory."""
+    if t.shape[0] > 1 and t.stride(0) < t[0].numel():
+        raise ValueError(f"{name} must not have rows that overlap")
+
+
+def lora_rows(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor, scale: Optional[torch.Tensor] = None,
+              base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a projection that they share (``gemm8``, ``mm8_m16``):
+    ``out[t] = base[t] + scale[i] * b[i] @ (a[i] @ x[t])`` with ``i = adapter[t]``.
+
+    ``x [T, n_in]`` and ``base [T, n_out]`` float32 or float64 (products and sums are computed in that type), ``a [N, R, n_in]``
+    and ``b [N, n_out, R]`` bfloat16, float16 or float32 with ``R <= 256`` (adapters of smaller rank are filled up with zeros),
+    ``adapter [T]`` int32: a row whose number is outside ``0..N-1`` has no adapter and gets ``base[t]``.  ``scale [N]`` float32;
+    without it 1.  ``base``: the shared projection's result, without it 0.  ``out`` may be ``base`` itself."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(a, torch.Tensor) or a.dim() != 3 or not isinstance(b, torch.Tensor) or b.dim() != 3:
+        raise ValueError("lora_rows: x must be [T, n_in], a [N, R, n_in], b [N, n_out, R]")
+    (T, n_in), (n, R, _), n_out, dev = x.shape, a.shape, b.shape[1], x.device
+    _is(x, (torch.float32, torch.float64), (T, n_in), "x")
+    _is(a, (torch.bfloat16, torch.float16, torch.float32), (n, R, n_in), "a", dev); _contig(a, "a")
+    _is(b, (a.dtype,), (n, n_out, R), "b", dev); _contig(b, "b")
+    _is(adapter, (torch.int32,), (T,), "adapter", dev); _contig(adapter, "adapter")
+    if scale is not None:
+        _is(scale, (torch.float32,), (n,), "scale", dev); _contig(scale, "scale")
+    if base is not None:
+        _is(base, (x.dtype,), (T, n_out), "base", dev)
+    out = torch.empty((T, n_out), dtype=x.dtype, device=dev) if out is None else out
+    _is(out, (x.dtype,), (T, n_out), "out", dev); _apart(out, "out")
+    strides = _rows(x, "x"), _rows(base, "base") if base is not None else 0, _rows(out, "out")
+    if T == 0:
+        return out
+    L, real = N.lib(), _TYPES[x.dtype]
+    ws = _workspace(L.rwkv_lora_rows_workspace_bytes(T, n_in, n_out, n, R, real), dev)
+    N.check(L.rwkv_lora_rows(_stream(), T, n_in, n_out, n, R, real, x.data_ptr(), strides[0], _TYPES[a.dtype], a.data_ptr(), b.data_ptr(),
+                             adapter.data_ptr(), scale.data_ptr() if scale is not None else None,
+                             base.data_ptr() if base is not None else None, strides[1], out.data_ptr(), strides[2], ws.data_ptr(), ws.numel()))
+    return out
+
+
+def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, state: torch.Tensor,
+               starts: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gated delta rule over packed sequences.  Per value head, row by row, with a state ``S [dk, dv]``:
+    ``S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = scale S^T q``.
+
+    ``q, k [T, Hk, dk]`` and ``v [T, Hv, dv]`` float32, bfloat16 or float16 (rows may be apart, heads are contiguous; ``dk <= 256``),
+    value head ``h`` with key head ``h // (Hv // Hk)``; ``g`` (logarithm of the decay, at most 0) and ``beta [T, Hv]`` float32;
+    ``state [B, Hv, dk, dv]`` float32, updated in place.  ``starts [B + 1]`` int32 on the device: sequence ``b`` is the rows
+    ``starts[b]`` to ``starts[b + 1] - 1``; without it ``T / B`` rows each.  ``scale``: ``dk ** -0.5`` unless given.
+    Returns ``o [T, Hv, dv]`` of v's type; rows of no sequence are not written, and an empty sequence keeps its state."""
+    for t, name in ((q, "q"), (v, "v")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3:
+            raise ValueError(f"delta_rule: {name} must be [T, heads, channels]")
+    if not isinstance(state, torch.Tensor) or state.dim() != 4:
+        raise ValueError("delta_rule: state must be [B, Hv, dk, dv]")
+    (T, Hk, dk), (_, Hv, dv), B, dev = q.shape, v.shape, state.shape[0], q.device
+    _is(q, (torch.float32, torch.bfloat16, torch.float16), (T, Hk, dk), "q")
+    _is(k, (q.dtype,), (T, Hk, dk), "k", dev); _is(v, (q.dtype,), (T, Hv, dv), "v", dev)
+    for t, name in ((g, "g"), (beta, "beta")):
+        _is(t, (torch.float32,), (T, Hv), name, dev); _contig(t, name)
+    _is(state, (torch.float32,), (B, Hv, dk, dv), "state", dev); _contig(state, "state")
+    if starts is not None:
+        _is(starts, (torch.int32,), (B + 1,), "starts", dev); _contig(starts, "starts")
+    elif B and T % B:
+        raise ValueError("delta_rule: without starts T must be a multiple of the sequences")
+    out = torch.empty((T, Hv, dv), dtype=q.dtype, device=dev) if out is None else out
+    _is(out, (q.dtype,), (T, Hv, dv), "out", dev); _contig(out, "out")
+    strides = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    if T == 0 or B == 0:
+        return out
+    L = N.lib()
+    ws = _workspace(L.rwkv_delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv), dev)
+    N.check(L.rwkv_delta_rule(_stream(), T, B, Hk, Hv, dk, dv, _TYPES[q.dtype], q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(),
+                              strides[2], g.data_ptr(), beta.data_ptr(), dk ** -0.5 if scale is None else float(scale),
+                              starts.data_ptr() if starts is not None else None, state.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel()))
+    return out
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: Optional[torch.Tensor] = None, *, draft_logits: Optional[torch.Tensor] = None,
+                  lengths: Optional[torch.Tensor] = None, temp: float = 1.0, greedy: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Drafted tokens held against the target's distribution (speculative sampling); returns ``(tokens [B, K+1], accepted [B])`` int64.
+
+    ``logits [B, K+1, V]`` float64 or float32: row ``i`` is the target's for the place of draft ``i`` (the logits after the token before
+    it), the last one for the token after all drafts; ``drafts [B, K]`` int64, of which the first ``lengths[b]`` (int32) count.  With
+    ``p = softmax(logits / temp)`` and ``q = softmax(draft_logits / temp)`` draft ``d`` is accepted while ``u[b, i] q(d) < p(d)``; at the
+    first refused one a token is drawn from ``max(p - q, 0)``, after the last from ``p``, by ``u[b, K]`` (``u [B, K+1]`` float32 in [0, 1)):
+    the lowest index at which the running weight exceeds ``u`` times the whole.  ``draft_logits [B, K, V]`` of logits' type; without them
+    the drafts have no distribution of their own (``q(d) = 1``).  ``greedy``: a draft is accepted while it is the first maximum, and the
+    token drawn is that maximum.  Row ``b`` of ``tokens`` is the accepted drafts, the token drawn, then -1 (there too, where no logit has weight)."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 3 or logits.shape[1] < 1:
+        raise ValueError("verify_drafts: logits must be [B, K + 1, V]")
+    (B, K1, V), dev = logits.shape, logits.device
+    _is(logits, (torch.float64, torch.float32), logits.shape, "logits")
+    _is(drafts, (torch.int64,), (B, K1 - 1), "drafts", dev); _contig(drafts, "drafts")
+    if draft_logits is not None:
+        _is(draft_logits, (logits.dtype,), (B, K1 - 1, V), "draft_logits", dev)
+    for t, name in ((logits, "logits"), (draft_logits, "draft_logits")):
+        if t is not None and t.numel() and t.stride(2) != 1 and V > 1:
+            raise ValueError(f"{name} must have contiguous rows")
+    if lengths is not None:
+        _is(lengths, (torch.int32,), (B,), "lengths", dev); _contig(lengths, "lengths")
+    if u is not None:
+        _is(u, (torch.float32,), (B, K1), "u", dev); _contig(u, "u")
+    elif not greedy:
+        raise ValueError("verify_drafts: u is needed unless greedy")
+    if not greedy and not temp > 0:
+        raise ValueError("verify_drafts: temp must be positive")
+    tokens, accepted = torch.empty((B, K1), dtype=torch.int64, device=dev), torch.empty(B, dtype=torch.int64, device=dev)
+    if B == 0:
+        return tokens, accepted
+    L = N.lib()
+    ws = _workspace(L.rwkv_verify_drafts_workspace_bytes(B, K1 - 1, V), dev)
+    opt = lambda t: t.data_ptr() if t is not None else None
+    by = draft_logits.stride() if draft_logits is not None else (0, 0)
+    N.check(L.rwkv_verify_drafts(_stream(), B, K1 - 1, V, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
+                                 opt(draft_logits), by[0], by[1], drafts.data_ptr(), opt(lengths), opt(u), float(temp), 1 if greedy else 0,
+                                 tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel()))
+    return tokens, accepted
