@@ -1,15 +1,29 @@
 // Drafted tokens held against the target's logits (rwkv_verify_drafts).  All arithmetic is float64: with 50277 tokens a running
 // sum in float32 would put one draw in a hundred on another token than the definition does.
+//
+// Each row of logits is cut into segments, at most kSegments of at least kChunk tokens:
+//   verify_rows_kernel  largest logit, and sum of the weights beside it (or first maximum), of every segment of every row
+//   verify_left_kernel  which drafts are accepted; where one is refused, the sums of what is left of its row, segment by segment
+//   verify_pick_kernel  the segment that the drawn token is in, and the token
+// Of the logits the first kernel reads everything once; the others read one row of each a sequence (from cache).
 #include "rwkv_types.h"
 
 namespace rwkv {
 
 namespace {
 
-constexpr int kVT = 256;             // threads
+constexpr int kVT = kThreads;        // threads of a workgroup
+constexpr int kPer = 16;             // tokens a thread takes at a time
+constexpr int kChunk = kVT * kPer;
+constexpr int kSegments = 64;
 constexpr int kMaxDrafts = 64;
 
-struct RowStat { double max, sum; int64_t first; };      // of a row: the largest logit, the sum of the weights, the first maximum (-1: none)
+struct RowStat { double max, sum; int first, pad; };     // of a segment: largest logit, sum of the weights beside it, first maximum (-1: none)
+
+struct Verdict {                     // of a sequence
+    double p_max, p_sum, q_max, q_sum;               // row n of both: the largest logit and the sum of the weights
+    int n, left;                                     // drafts accepted; whether q is taken off p
+};
 
 struct VerifyArgs {
     int64_t B, K, V;
@@ -19,116 +33,275 @@ struct VerifyArgs {
     const int32_t *lengths;
     const float *u;
     double inv_temp;
-    int greedy;
     int64_t *tokens, *accepted;
-    RowStat *stat;                   // [B][K+1], then [B][K] of the drafts' logits
+    int segments;
+    int64_t segment;                 // tokens of one, a multiple of kChunk
+    RowStat *stat;                   // [B][K+1][segments], then [B][K][segments] of the drafts' logits
+    double *sums;                    // [B][segments]
+    Verdict *verdict;                // [B]
 };
 
-// A logit's weight beside the row's largest; NaN and -infinity have none, and where the largest is +infinity the others have none.
+// A logit's weight beside the largest; NaN and -infinity have none, and where the largest is +infinity the others have none.
 __device__ __forceinline__ double weight(double x, double max, double inv_temp) {
-    if (!(x > -INFINITY)) return 0.0;
-    return x == max ? 1.0 : exp((x - max) * inv_temp);
+    const double d = (x - max) * inv_temp;
+    return d == d ? exp(d) : x == max && x > -INFINITY ? 1.0 : 0.0;
 }
 
-__device__ __forceinline__ void better(double &x, int64_t &i, double y, int64_t j) {
+__device__ __forceinline__ void better(double &x, int &i, double y, int j) {
     if (j >= 0 && (i < 0 || y > x || (y == x && j < i))) { x = y; i = j; }
 }
 
-// A workgroup per row.
-template <typename Real>
+template <typename Real> struct Wide;                // 16 bytes of logits, wherever a row starts
+template <> struct Wide<double> { typedef double type __attribute__((ext_vector_type(2), aligned(8))); };
+template <> struct Wide<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+
+// A workgroup per row and segment.
+template <typename Real, bool GREEDY>
 __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
+    using Vec = typename Wide<Real>::type;
+    constexpr int E = 16 / sizeof(Real);
     __shared__ double s_max[kWaves], red[kWaves];
-    __shared__ int64_t s_first[kWaves];
+    __shared__ int s_first[kWaves];
     const int64_t targets = a.B * (a.K + 1), at = blockIdx.x, of = at < targets ? a.K + 1 : a.K, row = at < targets ? at : at - targets;
     const Real *x = at < targets ? (const Real *)a.logits + row / of * a.seq + row % of * a.row
                                  : (const Real *)a.draft + row / of * a.draft_seq + row % of * a.draft_row;
-    double m = -INFINITY;
-    int64_t first = -1;
-    for (int64_t j = threadIdx.x; j < a.V; j += kVT) { const double y = x[j]; if (y > m) { m = y; first = j; } }
-    for (int off = 32; off >= 1; off >>= 1) better(m, first, __shfl_xor(m, off, 64), __shfl_xor((long long)first, off, 64));
-    if ((threadIdx.x & 63) == 0) { s_max[threadIdx.x >> 6] = m; s_first[threadIdx.x >> 6] = first; }
+    const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
+    double m = -INFINITY, s = 0.0;
+    int first = -1;
+    for (int64_t j = j0; j < j1; j += kChunk) {
+        Vec v[kPer / E];
+#pragma unroll
+        for (int k = 0; k < kPer / E; ++k) {
+            const int64_t i = j + (k * kVT + (int)threadIdx.x) * E;
+            if (i + E <= j1) v[k] = *reinterpret_cast<const Vec *>(x + i);
+            else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[k][e] = i + e < j1 ? x[i + e] : (Real)-INFINITY;
+            }
+        }
+        if (GREEDY) {
+#pragma unroll
+            for (int k = 0; k < kPer / E; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int i = (int)j + (k * kVT + (int)threadIdx.x) * E + e;
+                    if ((double)v[k][e] > m) { m = v[k][e]; first = i; }
+                }
+        } else {
+            double top = m;
+#pragma unroll
+            for (int k = 0; k < kPer / E; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) top = fmax(top, (double)v[k][e]);
+            s *= weight(m, top, a.inv_temp);
+            m = top;
+#pragma unroll
+            for (int k = 0; k < kPer / E; ++k)
+#pragma unroll
+                for (int e = 0; e < E; ++e) s += weight(v[k][e], m, a.inv_temp);
+        }
+    }
+    RowStat *to = a.stat + at * a.segments + blockIdx.y;
+    const double own = m;
+    if (GREEDY) {
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) better(m, first, __shfl_xor(m, off, 64), __shfl_xor(first, off, 64));
+        if ((threadIdx.x & 63) == 0) { s_max[threadIdx.x >> 6] = m; s_first[threadIdx.x >> 6] = first; }
+        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) better(m, first, s_max[w], s_first[w]);
+        if (threadIdx.x == 0) *to = {m, 0.0, first, 0};
+    } else {
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) m = fmax(m, __shfl_xor(m, off, 64));
+        if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) m = fmax(m, s_max[w]);
+        double sum[1] = {s * weight(own, m, a.inv_temp)};
+        block_sum(sum, red);
+        if (threadIdx.x == 0) *to = {m, sum[0], 0, 0};
+    }
+}
+
+// A row's segments put together.
+__device__ __forceinline__ void whole_row(const VerifyArgs &a, const RowStat *s, double &max, double &sum) {
+    max = -INFINITY; sum = 0.0;
+    for (int i = 0; i < a.segments; ++i) max = fmax(max, s[i].max);
+    for (int i = 0; i < a.segments; ++i) sum += s[i].sum * weight(s[i].max, max, a.inv_temp);
+}
+
+__device__ __forceinline__ int drafts_of(const VerifyArgs &a, int64_t b) { return a.lengths ? max(0, min((int)a.K, a.lengths[b])) : (int)a.K; }
+
+// What is left of p once q is taken off (or p itself) at tokens of one sequence's row n.
+template <typename Real>
+struct Left {
+    const Real *x, *y;
+    int64_t gone;                    // drafts without a distribution: the one that was refused
+    Verdict v;
+    double inv_temp;
+    __device__ Left(const VerifyArgs &a, int64_t b, const Verdict &v_) : v(v_), inv_temp(a.inv_temp) {
+        x = (const Real *)a.logits + b * a.seq + v.n * a.row;
+        y = a.draft && v.left ? (const Real *)a.draft + b * a.draft_seq + v.n * a.draft_row : nullptr;
+        gone = v.left ? a.drafts[b * a.K + v.n] : -1;
+    }
+    __device__ __forceinline__ double at(int64_t j) const {
+        const double p = weight(x[j], v.p_max, inv_temp) / v.p_sum;
+        if (!v.left) return p;
+        const double q = !y ? (j == gone ? 1.0 : 0.0) : v.q_sum > 0 ? weight(y[j], v.q_max, inv_temp) / v.q_sum : 0.0;
+        return fmax(p - q, 0.0);
+    }
+};
+
+// A workgroup per sequence and segment; each finds out for itself how many drafts are accepted, a thread to a draft.
+template <typename Real>
+__global__ void __launch_bounds__(kVT) verify_left_kernel(VerifyArgs a) {
+    __shared__ double red[kWaves];
+    __shared__ Verdict s_v;
+    const int64_t b = blockIdx.x;
+    const int tid = threadIdx.x, count = drafts_of(a, b);
+    const RowStat *ps = a.stat + b * (a.K + 1) * a.segments, *qs = a.stat + (a.B * (a.K + 1) + b * a.K) * a.segments;
+    if (tid < 64) {
+        bool taken = true;                            // (beyond the drafts nothing refuses)
+        if (tid < count) {
+            const int64_t d = a.drafts[b * a.K + tid];
+            taken = false;
+            if (d >= 0 && d < a.V) {
+                double max, sum, q = 1.0;
+                whole_row(a, ps + tid * a.segments, max, sum);
+                const double p = sum > 0 ? weight(((const Real *)a.logits)[b * a.seq + tid * a.row + d], max, a.inv_temp) / sum : 0.0;
+                if (a.draft) {
+                    whole_row(a, qs + tid * a.segments, max, sum);
+                    q = sum > 0 ? weight(((const Real *)a.draft)[b * a.draft_seq + tid * a.draft_row + d], max, a.inv_temp) / sum : 0.0;
+                }
+                taken = (double)a.u[b * (a.K + 1) + tid] * q < p;
+            }
+        }
+        const unsigned long long refused = __ballot(!taken);
+        const int n = refused ? min(__ffsll(refused) - 1, count) : count;
+        if (tid == 0) {
+            Verdict v{0, 0, -INFINITY, 0, n, n < count};
+            whole_row(a, ps + n * a.segments, v.p_max, v.p_sum);
+            if (v.left && a.draft) whole_row(a, qs + n * a.segments, v.q_max, v.q_sum);
+            s_v = v;
+            if (blockIdx.y == 0) a.verdict[b] = v;
+        }
+    }
     __syncthreads();
-    for (int w = 0; w < kWaves; ++w) better(m, first, s_max[w], s_first[w]);
+    const Verdict v = s_v;
+    if (!v.left || !(v.p_sum > 0)) return;
+    const Left<Real> left(a, b, v);
+    const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
     double s[1] = {0.0};
-    if (!a.greedy)
-        for (int64_t j = threadIdx.x; j < a.V; j += kVT) s[0] += weight(x[j], m, a.inv_temp);
+    for (int64_t j = j0; j < j1; j += kChunk) {
+#pragma unroll 4
+        for (int k = 0; k < kPer; ++k) {
+            const int64_t i = j + k * kVT + tid;
+            if (i < j1) s[0] += left.at(i);
+        }
+    }
     block_sum(s, red);
-    if (threadIdx.x == 0) a.stat[at] = {m, s[0], first};
+    if (tid == 0) a.sums[b * a.segments + blockIdx.y] = s[0];
+}
+
+// Accepted drafts, the token drawn, -1.
+__device__ __forceinline__ void answer(const VerifyArgs &a, int64_t b, int n, int64_t drawn) {
+    if (threadIdx.x <= a.K) a.tokens[b * (a.K + 1) + threadIdx.x] = threadIdx.x < n ? a.drafts[b * a.K + threadIdx.x] : threadIdx.x == n ? drawn : -1;
+    if (threadIdx.x == 0) a.accepted[b] = n;
 }
 
 // A workgroup per sequence.
 template <typename Real>
 __global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
-    __shared__ double sums[kVT], s_total;
-    __shared__ int s_n, s_count, s_any, s_pick;
+    __shared__ double s_sums[kSegments], s_wave[kWaves], s_aim, s_before;
+    __shared__ int s_segment, s_left, s_hit, s_last;
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x;
-    const Real *logits = (const Real *)a.logits + b * a.seq, *draft = a.draft ? (const Real *)a.draft + b * a.draft_seq : nullptr;
-    const RowStat *ps = a.stat + b * (a.K + 1), *qs = a.stat + a.B * (a.K + 1) + b * a.K;
-    if (tid == 0) {
-        const int count = a.lengths ? max(0, min((int)a.K, a.lengths[b])) : (int)a.K;
-        int n = 0;
-        for (; n < count; ++n) {
-            const int64_t d = a.drafts[b * a.K + n];
-            if (d < 0 || d >= a.V) break;
-            if (a.greedy) { if (ps[n].first != d) break; continue; }
-            const double p = ps[n].sum > 0 ? weight(logits[n * a.row + d], ps[n].max, a.inv_temp) / ps[n].sum : 0.0;
-            const double q = !draft ? 1.0 : qs[n].sum > 0 ? weight(draft[n * a.draft_row + d], qs[n].max, a.inv_temp) / qs[n].sum : 0.0;
-            if (!((double)a.u[b * (a.K + 1) + n] * q < p)) break;
+    Verdict v = a.verdict[b];
+    if (!(v.p_sum > 0)) { answer(a, b, v.n, -1); return; }
+    for (int round = v.left ? 0 : 1; round < 2; ++round) {              // what is left; p itself, where that is nothing
+        const RowStat *ps = a.stat + (b * (a.K + 1) + v.n) * a.segments;
+        __syncthreads();
+        if (tid < a.segments) s_sums[tid] = round == 0 ? a.sums[b * a.segments + tid] : ps[tid].sum * weight(ps[tid].max, v.p_max, a.inv_temp) / v.p_sum;
+        __syncthreads();
+        if (tid == 0) {
+            double all = 0.0, run = 0.0;
+            for (int i = 0; i < a.segments; ++i) all += s_sums[i];
+            const double aim = (double)a.u[b * (a.K + 1) + a.K] * all;
+            int at = -1;
+            for (int i = 0; i < a.segments; ++i) {                      // the first segment that passes the aim, or the last that has anything
+                if (s_sums[i] > 0.0) { at = i; s_before = run; }
+                run += s_sums[i];
+                if (run > aim && s_sums[i] > 0.0) break;
+            }
+            s_aim = aim; s_segment = at; s_left = round == 0; s_hit = 0x7fffffff; s_last = -1;
         }
-        s_n = n; s_count = count; s_pick = -1;
+        __syncthreads();
+        if (s_segment >= 0) break;
+    }
+    v.left = s_left;
+    const Left<Real> left(a, b, v);
+    const int64_t j0 = s_segment * a.segment, j1 = min(a.V, j0 + a.segment);
+    const double aim = s_aim;
+    double before = s_before;
+    for (int64_t j = j0; j < j1; j += kChunk) {                         // (one chunk, unless the vocabulary is over kSegments of them)
+        const int64_t i0 = j + tid * kPer;
+        double w[kPer], own = 0.0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) { w[k] = i0 + k < j1 ? left.at(i0 + k) : 0.0; own += w[k]; }
+        double run = own;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) { const double o = __shfl_up(run, off, 64); if ((tid & 63) >= off) run += o; }
+        if ((tid & 63) == 63) s_wave[tid >> 6] = run;
+        __syncthreads();
+        double after = before;
+        run += before - own;
+#pragma unroll
+        for (int q = 0; q < kWaves; ++q) { run += q < (tid >> 6) ? s_wave[q] : 0.0; after += s_wave[q]; }
+        int hit = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            run += w[k];
+            if (w[k] > 0.0) { last = (int)(i0 + k); if (run > aim && hit == 0x7fffffff) hit = last; }
+        }
+        if (hit != 0x7fffffff) atomicMin(&s_hit, hit);
+        if (last >= 0) atomicMax(&s_last, last);
+        __syncthreads();
+        if (s_hit != 0x7fffffff) break;
+        before = after;
+    }
+    answer(a, b, v.n, s_hit != 0x7fffffff ? s_hit : s_last);            // (rounding can leave none over the aim: the segment's last that has weight)
+}
+
+// A wavefront per sequence, a lane to a row.
+__global__ void __launch_bounds__(kMaxDrafts + 64) verify_greedy_kernel(VerifyArgs a) {
+    __shared__ int best[kMaxDrafts + 1];
+    const int64_t b = blockIdx.x;
+    const int tid = threadIdx.x, count = drafts_of(a, b);
+    if (tid <= a.K) {
+        const RowStat *s = a.stat + (b * (a.K + 1) + tid) * a.segments;
+        double m = -INFINITY;
+        int first = -1;
+        for (int i = 0; i < a.segments; ++i) better(m, first, s[i].max, s[i].first);
+        best[tid] = first;
     }
     __syncthreads();
-    const int n = s_n;
-    int64_t pick = -1;
-    if (a.greedy) pick = ps[n].first;
-    else if (ps[n].sum > 0) {
-        const Real *x = logits + n * a.row, *y = draft ? draft + n * a.draft_row : nullptr;
-        const int64_t gone = n < s_count ? a.drafts[b * a.K + n] : -1;
-        bool left = n < s_count;                      // what is left of p once q is taken off, or p itself
-        const int64_t per = ceil_div(a.V, kVT), j0 = min(a.V, per * tid), j1 = min(a.V, j0 + per);
-        auto value = [&](int64_t j) {
-            const double p = weight(x[j], ps[n].max, a.inv_temp) / ps[n].sum;
-            if (!left) return p;
-            const double q = !y ? (j == gone ? 1.0 : 0.0) : qs[n].sum > 0 ? weight(y[j], qs[n].max, a.inv_temp) / qs[n].sum : 0.0;
-            return fmax(p - q, 0.0);
-        };
-        for (;;) {
-            double s = 0.0;
-            for (int64_t j = j0; j < j1; ++j) s += value(j);
-            __syncthreads();
-            sums[tid] = s;
-            if (tid == 0) s_any = 0;
-            __syncthreads();
-            if (tid == 0) {
-                double run = 0.0;
-                for (int i = 0; i < kVT; ++i) { const double v = sums[i]; sums[i] = run; run += v; }
-                s_total = run;
-            }
-            __syncthreads();
-            if (s_total > 0.0 || !left) break;
-            left = false;
-        }
-        // the lowest index whose running weight is over the aim; rounding can leave none: then the last one that has weight
-        const double aim = (double)a.u[b * (a.K + 1) + a.K] * s_total;
-        double run = sums[tid];
-        int last = -1, hit = -1;
-        for (int64_t j = j0; j < j1 && hit < 0; ++j) {
-            const double w = value(j);
-            run += w;
-            if (w > 0.0) { last = (int)j; if (run > aim) hit = (int)j; }
-        }
-        __shared__ int s_hit;
-        if (tid == 0) s_hit = 0x7fffffff;
-        __syncthreads();
-        if (hit >= 0) atomicMin(&s_hit, hit);
-        if (last >= 0) atomicMax(&s_pick, last);
-        __syncthreads();
-        pick = s_hit != 0x7fffffff ? s_hit : s_pick;
-    }
-    for (int64_t i = tid; i <= a.K; i += kVT) a.tokens[b * (a.K + 1) + i] = i < n ? a.drafts[b * a.K + i] : i == n ? pick : -1;
-    if (tid == 0) a.accepted[b] = n;
+    int n = 0;
+    while (n < count && best[n] >= 0 && best[n] == a.drafts[b * a.K + n]) ++n;
+    answer(a, b, n, best[n]);
 }
+
+struct VerifyPlan {
+    int segments;
+    int64_t segment;
+    size_t stat_bytes, sum_bytes, verdict_bytes;
+    VerifyPlan(int64_t B, int64_t K, int64_t V) {
+        segment = round_up(ceil_div(V, kSegments), kChunk);
+        segments = (int)ceil_div(V, segment);
+        stat_bytes = (size_t)(B * (2 * K + 1) * segments) * sizeof(RowStat);
+        sum_bytes = (size_t)(B * segments) * 8;
+        verdict_bytes = (size_t)B * sizeof(Verdict);
+    }
+    size_t bytes() const { return stat_bytes + sum_bytes + verdict_bytes; }
+};
 
 }  // namespace
 
@@ -140,7 +313,7 @@ extern "C" {
 
 size_t rwkv_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V) {
     if (B <= 0 || K < 0 || V <= 0) return 0;
-    return (size_t)(B * (2 * K + 1)) * sizeof(RowStat);
+    return VerifyPlan(B, K, V).bytes();
 }
 
 int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, int real, const void *logits, int64_t logits_seq_stride,
@@ -154,15 +327,25 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
     RWKV_CHECK_ARG(logits_seq_stride >= 0 && logits_row_stride >= 0 && draft_seq_stride >= 0 && draft_row_stride >= 0, "rwkv_verify_drafts: negative stride");
     if (K > kMaxDrafts || V >= (1ll << 31) || B >= (1ll << 24)) return set_error(RWKV_ERR_SIZE, "rwkv_verify_drafts: at most %d drafts", kMaxDrafts);
     RWKV_CHECK_ALIGN(workspace, 16);
-    if (!workspace || workspace_bytes < rwkv_verify_drafts_workspace_bytes(B, K, V))
-        return set_error(RWKV_ERR_WORKSPACE, "rwkv_verify_drafts: workspace too small");
+    const VerifyPlan pl(B, K, V);
+    if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_verify_drafts: workspace too small");
+    uint8_t *ws = (uint8_t *)workspace;
     const bool of_drafts = draft_logits && !greedy && K > 0;
     const VerifyArgs a{B, K, V, logits, logits_seq_stride, logits_row_stride, of_drafts ? draft_logits : nullptr, draft_seq_stride, draft_row_stride,
-                       drafts, lengths, u, 1.0 / temp, greedy != 0, tokens, accepted, (RowStat *)workspace};
+                       drafts, lengths, u, 1.0 / temp, tokens, accepted, pl.segments, pl.segment, (RowStat *)ws, (double *)(ws + pl.stat_bytes),
+                       (Verdict *)(ws + pl.stat_bytes + pl.sum_bytes)};
+    const hipStream_t st = (hipStream_t)stream;
+    const dim3 rows((unsigned)(B * (K + 1) + (of_drafts ? B * K : 0)), (unsigned)pl.segments), left((unsigned)B, (unsigned)pl.segments);
     with_real(real, [&](auto re) {
         using Real = typename decltype(re)::type;
-        hipLaunchKernelGGL(verify_rows_kernel<Real>, dim3((unsigned)(B * (K + 1) + (of_drafts ? B * K : 0))), dim3(kVT), 0, (hipStream_t)stream, a);
-        hipLaunchKernelGGL(verify_pick_kernel<Real>, dim3((unsigned)B), dim3(kVT), 0, (hipStream_t)stream, a);
+        if (greedy) {
+            hipLaunchKernelGGL((verify_rows_kernel<Real, true>), rows, dim3(kVT), 0, st, a);
+            hipLaunchKernelGGL(verify_greedy_kernel, dim3((unsigned)B), dim3(kMaxDrafts + 64), 0, st, a);
+        } else {
+            hipLaunchKernelGGL((verify_rows_kernel<Real, false>), rows, dim3(kVT), 0, st, a);
+            hipLaunchKernelGGL(verify_left_kernel<Real>, left, dim3(kVT), 0, st, a);
+            hipLaunchKernelGGL(verify_pick_kernel<Real>, dim3((unsigned)B), dim3(kVT), 0, st, a);
+        }
     });
     RWKV_CHECK_LAUNCH("verify_pick_kernel");
     return RWKV_OK;
