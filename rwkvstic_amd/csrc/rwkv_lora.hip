@@ -17,7 +17,7 @@ namespace {
 constexpr int kDirect = 256;          // most rows whose tiles the wavefronts find for themselves
 constexpr int kWindow = 1024;         // rows sorted together by lora_plan_kernel: a thread each
 constexpr int kSlices = 8;            // most slices of n_in
-constexpr int kStep = 32;             // outputs a wavefront of lora_up_kernel makes at once
+constexpr int kDownWaves = 8;         // wavefronts of lora_down_kernel: parts of a slice
 
 struct Tile { int first, n, adapter; };          // rows order[first .. first + n - 1]
 
@@ -29,7 +29,8 @@ struct LoraArgs {
     const float *scale;
     const void *base; int64_t base_stride;
     void *out; int64_t out_stride;
-    int slices, steps, range;             // slices of n_in, blocks of 32 in a quarter of each; outputs of a workgroup
+    int slices, steps, range;             // slices of n_in, blocks of 32 in a wavefront's part of each; outputs of a workgroup
+    int chunks;                           // ranges, filled up to whole rounds of the XCDs
     int ranks;                            // R filled up to what the kernels' tiles hold
     void *h;                              // [slices][T][ranks]
     int32_t *order;                       // rows by window and adapter, or null: tiles are found directly
@@ -64,6 +65,69 @@ __device__ __forceinline__ void load8(Eight<T> &to, const T *row, int64_t k, int
         for (int i = 0; i < 8; ++i) to.e[i] = k + i < n ? row[k + i] : (T)0.f;
     }
 }
+
+// What the matrix instructions make of eight terms (32 with the other lanes'): left operand from an adapter, right one from x or h.
+// In LDS the right operands of a row of n lie in planes [rows][n + pad]; the pad leaves rows an odd number of 16 bytes apart.
+template <typename Real, typename Low> struct Product {
+    using Vec = typename Four<Real>::type;
+    using Right = Eight<Real>;
+    static constexpr int kPad = 16 / sizeof(Real);
+    static constexpr int row_bytes(int n) { return (n + kPad) * sizeof(Real); }
+    static __device__ __forceinline__ Right right(const Eight<Real> &v) { return v; }
+    static __device__ __forceinline__ void put(unsigned char *lds, int rows, int n, int row, int k, const Vec &v) {
+        *reinterpret_cast<Vec *>(reinterpret_cast<Real *>(lds) + row * (n + kPad) + k) = v;
+    }
+    static __device__ __forceinline__ Right get(const unsigned char *lds, int rows, int n, int row, int k) {
+        Right r;
+        load8<true>(r, reinterpret_cast<const Real *>(lds) + row * (n + kPad), k, n);
+        return r;
+    }
+    static __device__ __forceinline__ void add(Vec &acc, const Eight<Low> &l, const Right &r) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc = mfma((Real)l.e[e], r.e[e], acc);
+    }
+};
+
+// float32 rows and bfloat16 adapters: a float32 value is the sum of three bfloat16 ones, its 24 bits cut in three, so that three
+// bfloat16 products with float32 sums lose nothing, in a fifth of the matrix cores' time for float32 operands.
+template <> struct Product<float, __bf16> {
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    using Vec = f32x4;
+    struct Right { u32x4 part[3]; };
+    static constexpr int kPad = 8;
+    static constexpr int row_bytes(int n) { return 3 * (n + kPad) * 2; }
+    static __device__ __forceinline__ float rest(float v) { return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+    static __device__ __forceinline__ uint32_t upper(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+    static __device__ __forceinline__ Right right(const Eight<float> &v) {
+        Right r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float a = v.e[2 * i], b = v.e[2 * i + 1], a1 = rest(a), b1 = rest(b);
+            r.part[0][i] = upper(a, b); r.part[1][i] = upper(a1, b1); r.part[2][i] = upper(rest(a1), rest(b1));
+        }
+        return r;
+    }
+    static __device__ __forceinline__ void put(unsigned char *lds, int rows, int n, int row, int k, const Vec &v) {
+        float f[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            *reinterpret_cast<uint2 *>(lds + ((part * rows + row) * (n + kPad) + k) * 2) = make_uint2(upper(f[0], f[1]), upper(f[2], f[3]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = rest(f[i]);
+        }
+    }
+    static __device__ __forceinline__ Right get(const unsigned char *lds, int rows, int n, int row, int k) {
+        Right r;
+#pragma unroll
+        for (int part = 0; part < 3; ++part) r.part[part] = *reinterpret_cast<const u32x4 *>(lds + ((part * rows + row) * (n + kPad) + k) * 2);
+        return r;
+    }
+    static __device__ __forceinline__ void add(Vec &acc, const Eight<__bf16> &l, const Right &r) {
+#pragma unroll
+        for (int part = 2; part >= 0; --part)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, l.part[0]), __builtin_bit_cast(bf16x8, r.part[part]), acc, 0, 0, 0);
+    }
+};
 
 // The tile of a workgroup: its rows in `rows` (LDS, 64 at most).  false: this workgroup has none.  Directly: slot t has a tile if the
 // rows before t hold a multiple of 16 with t's adapter; it is t and the next 15 of them.
@@ -146,145 +210,184 @@ __global__ void __launch_bounds__(kWindow) lora_plan_kernel(LoraArgs p, int slot
     for (int i = all + tid; i < slots; i += kWindow) to[i] = {0, 0, -1};
 }
 
-// A workgroup to 16 rows, RT tiles of 16 ranks and a slice of n_in, of which each wavefront takes a quarter.
-template <typename Real, typename Low, int RT, bool WIDE>
-__global__ void __launch_bounds__(256) lora_down_kernel(LoraArgs p) {
-    using Vec = typename Four<Real>::type;
+// A workgroup to NT times 16 rows, RT tiles of 16 ranks and a slice of n_in, of which each wavefront takes a part, with the
+// loads of the next 32 terms under way.  Neighbouring workgroups (on different XCDs) have different slices, so that an XCD's L2
+// holds its slices of a.
+template <typename Real, typename Low, int RT, int NT, bool WIDE>
+__global__ void __launch_bounds__(64 * kDownWaves) lora_down_kernel(LoraArgs p) {
+    using Op = Product<Real, Low>;
+    using Vec = typename Op::Vec;
     __shared__ int rows[64];
-    __shared__ Vec sums[3][RT][64];
-    const int parts = p.order ? 4 : 1, part = blockIdx.x % parts, rank0 = blockIdx.z * RT * 16;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Vec *sums = reinterpret_cast<Vec *>(smem);        // [kDownWaves / 2][NT * RT][64]
+    constexpr int kParts = 4 / NT;
+    const int slice = blockIdx.x % p.slices, place = blockIdx.x / p.slices, parts = p.order ? kParts : 1;
+    const int row0 = place % parts * NT * 16, rank0 = blockIdx.z * RT * 16;
     Tile tile;
-    if (!find_tile(p, blockIdx.x / parts, tile, rows) || tile.adapter < 0 || part * 16 >= tile.n) return;
+    if (!find_tile(p, place / parts, tile, rows) || tile.adapter < 0 || row0 >= tile.n) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int64_t t = rows[min(part * 16 + i, tile.n - 1)];
-    const Real *x = (const Real *)p.x + t * p.x_stride;
+    const Real *x[NT];
+#pragma unroll
+    for (int s = 0; s < NT; ++s) x[s] = (const Real *)p.x + (int64_t)rows[min(row0 + s * 16 + i, tile.n - 1)] * p.x_stride;
     const Low *a[RT];
 #pragma unroll
     for (int q = 0; q < RT; ++q)              // (ranks past the last: the last again, what comes of it is dropped)
         a[q] = (const Low *)p.a + ((int64_t)tile.adapter * p.R + min(rank0 + q * 16 + left_row<Real>(i), (int)p.R - 1)) * p.n_in;
-    Vec acc[RT];
+    Vec acc[NT][RT];
 #pragma unroll
-    for (int q = 0; q < RT; ++q) acc[q] = Vec{0, 0, 0, 0};
-    const int64_t k0 = ((int64_t)blockIdx.y * 4 + wave) * p.steps * 32, k1 = min(p.n_in, k0 + (int64_t)p.steps * 32);
-    Eight<Real> xv;
-    Eight<Low> av[RT];
-    auto load = [&](int64_t k) {
-        load8<WIDE>(xv, x, k, k1);
+    for (int s = 0; s < NT; ++s)
 #pragma unroll
-        for (int q = 0; q < RT; ++q) load8<WIDE>(av[q], a[q], k, k1);
+        for (int q = 0; q < RT; ++q) acc[s][q] = Vec{0, 0, 0, 0};
+    const int64_t k0 = ((int64_t)slice * kDownWaves + wave) * p.steps * 32, k1 = min(p.n_in, k0 + (int64_t)p.steps * 32);
+    struct Terms { Eight<Real> x[NT]; Eight<Low> a[RT]; };
+    auto load = [&](Terms &v, int64_t k) {
+        if (k >= k1) return;
+#pragma unroll
+        for (int s = 0; s < NT; ++s) load8<WIDE>(v.x[s], x[s], k + 8 * g, k1);
+#pragma unroll
+        for (int q = 0; q < RT; ++q) load8<WIDE>(v.a[q], a[q], k + 8 * g, k1);
     };
-    if (k0 < k1) load(k0 + 8 * g);
-    for (int64_t k = k0; k < k1; k += 32) {
-        const Eight<Real> xn = xv;
-        Eight<Low> an[RT];
+    auto multiply = [&](const Terms &v) {
 #pragma unroll
-        for (int q = 0; q < RT; ++q) an[q] = av[q];
-        if (k + 32 < k1) load(k + 32 + 8 * g);
+        for (int s = 0; s < NT; ++s) {
+            const typename Op::Right r = Op::right(v.x[s]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int q = 0; q < RT; ++q) acc[q] = mfma((Real)an[q].e[e], xn.e[e], acc[q]);
+            for (int q = 0; q < RT; ++q) Op::add(acc[s][q], v.a[q], r);
+        }
+    };
+    Terms even, odd;
+    load(even, k0);
+    for (int64_t k = k0; k < k1; k += 64) {
+        load(odd, k + 32);
+        multiply(even);
+        load(even, k + 64);
+        if (k + 32 < k1) multiply(odd);
     }
-    if (wave)
 #pragma unroll
-        for (int q = 0; q < RT; ++q) sums[wave - 1][q][lane] = acc[q];
-    __syncthreads();
-    if (wave || part * 16 + i >= tile.n) return;
+    for (int half = kDownWaves / 2; half >= 1; half /= 2) {
+        if (half < kDownWaves / 2) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NT * RT; ++c)
+            if (wave >= half && wave < 2 * half) sums[((wave - half) * NT * RT + c) * 64 + lane] = acc[c / RT][c % RT];
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NT * RT; ++c)
+            if (wave < half) acc[c / RT][c % RT] += sums[(wave * NT * RT + c) * 64 + lane];
+    }
+    if (wave) return;
     const Real scale = p.scale ? (Real)p.scale[tile.adapter] : (Real)1;
-    Real *h = (Real *)p.h + ((int64_t)blockIdx.y * p.T + t) * p.ranks + rank0 + 4 * g;
 #pragma unroll
-    for (int q = 0; q < RT; ++q) {
-        const Vec s = ((acc[q] + sums[0][q][lane]) + sums[1][q][lane]) + sums[2][q][lane];
-        Vec v;
+    for (int s = 0; s < NT; ++s) {
+        if (row0 + s * 16 + i >= tile.n) break;
+        Real *h = (Real *)p.h + ((int64_t)slice * p.T + rows[row0 + s * 16 + i]) * p.ranks + rank0 + 4 * g;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = rank0 + q * 16 + 4 * g + c < p.R ? s[c] * scale : (Real)0;
-        *reinterpret_cast<Vec *>(h + q * 16) = v;
+        for (int q = 0; q < RT; ++q) {
+            Vec v = acc[s][q];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] = rank0 + q * 16 + 4 * g + c < p.R ? v[c] * scale : (Real)0;
+            *reinterpret_cast<Vec *>(h + q * 16) = v;
+        }
     }
 }
 
-// RB blocks of 32 ranks, NT times 16 rows of the tile: as many as 64 KiB of LDS hold.
-template <typename Real, typename Low, int RB, int NT, bool WIDE>
+// RB blocks of 32 ranks, NT times 16 rows of the tile: as many as 64 KiB of LDS hold.  An XCD takes the same ranges of outputs
+// for all tiles, and so reads these rows of b once.
+template <typename Real, typename Low, int RB, int NT, int QT, bool WIDE>
 __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
-    using Vec = typename Four<Real>::type;
-    constexpr int kPad = 16 / sizeof(Real), kRow = RB * 32 + kPad;              // rows 16 bytes apart in the banks
-    extern __shared__ __align__(16) unsigned char smem[];
-    Real *hs = reinterpret_cast<Real *>(smem);                                  // [NT * 16][kRow]
+    using Op = Product<Real, Low>;
+    using Vec = typename Op::Vec;
+    extern __shared__ __align__(16) unsigned char hs[];                        // right operands of the tile's rows
     __shared__ int rows[64];
     Tile tile;
     const int row0 = blockIdx.z * NT * 16;
-    if (!find_tile(p, blockIdx.x, tile, rows) || row0 >= tile.n) return;
+    const int64_t n0 = (int64_t)(blockIdx.x % p.chunks) * p.range, n1 = min(p.n_out, n0 + p.range);
+    if (n0 >= n1 || !find_tile(p, blockIdx.x / p.chunks, tile, rows) || row0 >= tile.n) return;
     const int n_rows = min(NT * 16, tile.n - row0);
-    const int64_t n0 = (int64_t)blockIdx.y * p.range, n1 = min(p.n_out, n0 + p.range);
     const Real *base = (const Real *)p.base;
     Real *out = (Real *)p.out;
     if (tile.adapter < 0) {                           // rows without an adapter
         if (out == base && p.out_stride == p.base_stride) return;
-        for (int r = row0; r < row0 + n_rows; ++r)
-            for (int64_t n = n0 + threadIdx.x; n < n1; n += 256)
-                out[(int64_t)rows[r] * p.out_stride + n] = base ? base[(int64_t)rows[r] * p.base_stride + n] : (Real)0;
+        constexpr int E = WIDE ? 16 / sizeof(Real) : 1;
+        typedef Real Some __attribute__((ext_vector_type(E)));
+        const int wide = (int)((n1 - n0) / E);
+#pragma unroll 4
+        for (int at = threadIdx.x; at < n_rows * wide; at += 256) {
+            const int64_t t = rows[row0 + at / wide], n = n0 + at % wide * E;
+            *reinterpret_cast<Some *>(out + t * p.out_stride + n) = base ? *reinterpret_cast<const Some *>(base + t * p.base_stride + n) : Some(0);
+        }
         return;
     }
-    for (int i = threadIdx.x; i < n_rows * RB * 8; i += 256) {
-        const int r = i / (RB * 8), c = i % (RB * 8) * 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const Low *b = (const Low *)p.b + (int64_t)tile.adapter * p.n_out * p.R;
+    // QT tiles of outputs: lane (j, g) comes out with n + 16 q + 4 g .. + 3 of row j, 64 bytes of a row (128 of float64) to a store
+    struct Rows { Eight<Low> v[QT][RB]; };
+    auto load = [&](Rows &to, int64_t n) {
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            const Low *row = b + min(n + 16 * q + left_row<Real>(i), p.n_out - 1) * p.R;
+#pragma unroll
+            for (int k = 0; k < RB; ++k) load8<WIDE>(to.v[q][k], row, k * 32 + 8 * g, p.R);
+        }
+    };
+    struct Onto { Vec v[QT]; };
+    auto load_base = [&](Onto &to, int s, int64_t n) {
+#pragma unroll
+        for (int q = 0; q < QT; ++q) to.v[q] = Vec{0, 0, 0, 0};
+        if (!base || s * 16 + i >= n_rows) return;
+        const Real *from = base + (int64_t)rows[row0 + s * 16 + i] * p.base_stride + n + 4 * g;
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+            if (WIDE) { if (n + 4 * g + 16 * q < n1) to.v[q] = *reinterpret_cast<const Vec *>(from + 16 * q); }
+            else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) if (n + 4 * g + 16 * q + c < n1) to.v[q][c] = from[16 * q + c];
+            }
+        }
+    };
+    Rows now;
+    int64_t n = n0 + wave * 16 * QT;
+    load(now, n);
+    for (int at = threadIdx.x; at < n_rows * RB * 8; at += 256) {
+        const int r = at / (RB * 8), c = at % (RB * 8) * 4;
         const Real *h = (const Real *)p.h + (int64_t)rows[row0 + r] * p.ranks + c;
         Vec s = *reinterpret_cast<const Vec *>(h);
 #pragma unroll 4
         for (int k = 1; k < p.slices; ++k) s += *reinterpret_cast<const Vec *>(h + k * p.T * p.ranks);
-        *reinterpret_cast<Vec *>(hs + r * kRow + c) = s;
+        Op::put(hs, NT * 16, RB * 32, r, c, s);
     }
     __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const Low *b = (const Low *)p.b + (int64_t)tile.adapter * p.n_out * p.R;
-    for (int64_t n = n0 + wave * kStep; n < n1; n += 4 * kStep) {
-        // two tiles of outputs, in an order that leaves each lane with the eight n + 8 g .. n + 8 g + 7
-        Eight<Low> bv[2][RB];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int l = left_row<Real>(i);
-            const Low *row = b + min(n + 8 * (l >> 2) + 4 * q + (l & 3), n1 - 1) * p.R;
-#pragma unroll
-            for (int k = 0; k < RB; ++k) load8<WIDE>(bv[q][k], row, k * 32 + 8 * g, p.R);
-        }
+    while (n < n1) {
+        Onto onto, ahead;
+        load_base(onto, 0, n);
 #pragma unroll
         for (int s = 0; s < NT; ++s) {
             if (s * 16 >= n_rows) break;
-            const bool in = s * 16 + i < n_rows;
-            const int64_t t = rows[row0 + min(s * 16 + i, n_rows - 1)];
-            Vec acc[2];
+            if (s + 1 < NT) load_base(ahead, s + 1, n);
+            Vec acc[QT];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int64_t at = n + 8 * g + 4 * q;
-                acc[q] = Vec{0, 0, 0, 0};
-                if (base && in) {
-                    const Real *from = base + t * p.base_stride + at;
-                    if (WIDE) { if (at < n1) acc[q] = *reinterpret_cast<const Vec *>(from); }
+            for (int q = 0; q < QT; ++q) acc[q] = Vec{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < RB; ++k) {
+                const typename Op::Right r = Op::get(hs, NT * 16, RB * 32, s * 16 + i, k * 32 + 8 * g);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) Op::add(acc[q], now.v[q][k], r);
+            }
+            if (s * 16 + i < n_rows) {
+                Real *to = out + (int64_t)rows[row0 + s * 16 + i] * p.out_stride + n + 4 * g;
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    acc[q] += onto.v[q];
+                    if (WIDE) { if (n + 4 * g + 16 * q < n1) *reinterpret_cast<Vec *>(to + 16 * q) = acc[q]; }
                     else {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) if (at + c < n1) acc[q][c] = from[c];
+                        for (int c = 0; c < 4; ++c) if (n + 4 * g + 16 * q + c < n1) to[16 * q + c] = acc[q][c];
                     }
                 }
             }
-#pragma unroll
-            for (int k = 0; k < RB; ++k) {
-                Eight<Real> hv;
-                load8<true>(hv, hs + (s * 16 + i) * kRow, k * 32 + 8 * g, RB * 32);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) acc[q] = mfma((Real)bv[q][k].e[e], hv.e[e], acc[q]);
-            }
-            if (!in) continue;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int64_t at = n + 8 * g + 4 * q;
-                Real *to = out + t * p.out_stride + at;
-                if (WIDE) { if (at < n1) *reinterpret_cast<Vec *>(to) = acc[q]; }
-                else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) if (at + c < n1) to[c] = acc[q][c];
-                }
-            }
+            onto = ahead;
         }
+        n += 4 * 16 * QT;
+        if (n < n1) load(now, n);
     }
 }
 
@@ -293,7 +396,7 @@ struct LoraPlan {
     bool direct;
     int windows, slots;                   // tiles are looked for in windows * slots places
     int group, groups, ranks;             // tiles of 16 ranks to a wavefront of lora_down_kernel, and wavefronts
-    int slices, steps, range;
+    int slices, steps, range, chunks;
     size_t h_bytes, order_bytes, tile_bytes;
     LoraPlan(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real) {
         direct = T <= kDirect;
@@ -303,12 +406,14 @@ struct LoraPlan {
         groups = (int)ceil_div(R, group * 16);
         ranks = group * groups * 16;
         const int64_t blocks = ceil_div(n_in, 32), tiles = direct ? T : ceil_div(T, 16);
-        int64_t s = ceil_div(512, tiles);
-        s = s < 1 ? 1 : s > kSlices ? kSlices : s;
-        steps = (int)ceil_div(blocks, 4 * s);
-        slices = (int)ceil_div(blocks, 4 * steps);
-        const int64_t chunks = ceil_div(direct ? 1024 : 2048, direct ? T : ceil_div(T, 64));
-        range = (int)round_up(ceil_div(n_out, chunks), 4 * kStep);
+        int64_t s = 1;
+        while (s < kSlices && s * tiles < (direct ? 256 : 512) && blocks > s * kDownWaves) s *= 2;
+        steps = (int)ceil_div(blocks, kDownWaves * s);
+        slices = (int)ceil_div(blocks, kDownWaves * steps);
+        const int64_t wanted = ceil_div(direct ? 2048 : 1024, direct ? T : ceil_div(T, 64));
+        range = (int)round_up(ceil_div(n_out, wanted), direct || real == RWKV_F64 ? 128 : 256);
+        chunks = (int)ceil_div(n_out, range);
+        if (chunks > 8) chunks = (int)round_up(chunks, 8);
         h_bytes = round_up((size_t)slices * T * ranks * type_bytes(real), 256);
         order_bytes = direct ? 0 : round_up((size_t)T * 4, 256);
         tile_bytes = direct ? 0 : (size_t)windows * slots * sizeof(Tile);
@@ -318,22 +423,29 @@ struct LoraPlan {
 
 template <typename Real, typename Low, bool WIDE>
 void launch(hipStream_t st, const LoraPlan &pl, const LoraArgs &p) {
+    using Op = Product<Real, Low>;
     const int places = pl.windows * pl.slots;
-    const dim3 down((unsigned)(places * (pl.direct ? 1 : 4)), (unsigned)pl.slices, (unsigned)pl.groups);
-    auto go_down = [&](auto k) { hipLaunchKernelGGL(k, down, dim3(256), 0, st, p); };
-    if (pl.group == 2) go_down(lora_down_kernel<Real, Low, 2, WIDE>);
-    else if (pl.group == 4) go_down(lora_down_kernel<Real, Low, 4, WIDE>);
-    else go_down(lora_down_kernel<Real, Low, 8, WIDE>);
+    // 32 rows of lora_down_kernel read the same of a, where that many can be in a tile and their sums stay in registers
+    constexpr int kMany = sizeof(Real) == 4 ? 2 : 1;
+    auto go_down = [&](auto one, auto many, int group) {
+        const int nt = pl.direct ? 1 : kMany;
+        const dim3 down((unsigned)(places * (pl.direct ? 1 : 4 / nt) * pl.slices), 1, (unsigned)pl.groups);
+        hipLaunchKernelGGL(pl.direct ? one : many, down, dim3(64 * kDownWaves), (size_t)kDownWaves / 2 * nt * group * 64 * 4 * sizeof(Real), st, p);
+    };
+    if (pl.group == 2) go_down(lora_down_kernel<Real, Low, 2, 1, WIDE>, lora_down_kernel<Real, Low, 2, kMany, WIDE>, 2);
+    else if (pl.group == 4) go_down(lora_down_kernel<Real, Low, 4, 1, WIDE>, lora_down_kernel<Real, Low, 4, kMany, WIDE>, 4);
+    else go_down(lora_down_kernel<Real, Low, 8, 1, WIDE>, lora_down_kernel<Real, Low, 8, kMany, WIDE>, 8);
     auto go_up = [&](auto one, auto many, int nt) {
         const int rows = 16 * (pl.direct ? 1 : nt);
-        const dim3 up((unsigned)places, (unsigned)ceil_div(p.n_out, pl.range), (unsigned)(pl.direct ? 1 : 4 / nt));
-        hipLaunchKernelGGL(pl.direct ? one : many, up, dim3(256), (size_t)rows * (pl.ranks * sizeof(Real) + 16), st, p);
+        const dim3 up((unsigned)(places * pl.chunks), 1, (unsigned)(pl.direct ? 1 : 4 / nt));
+        hipLaunchKernelGGL(pl.direct ? one : many, up, dim3(256), (size_t)rows * Op::row_bytes(pl.ranks), st, p);
     };
-    constexpr int k128 = sizeof(Real) == 4 ? 4 : 2, k256 = k128 / 2;
-    if (pl.ranks == 32) go_up(lora_up_kernel<Real, Low, 1, 1, WIDE>, lora_up_kernel<Real, Low, 1, 4, WIDE>, 4);
-    else if (pl.ranks == 64) go_up(lora_up_kernel<Real, Low, 2, 1, WIDE>, lora_up_kernel<Real, Low, 2, 4, WIDE>, 4);
-    else if (pl.ranks == 128) go_up(lora_up_kernel<Real, Low, 4, 1, WIDE>, lora_up_kernel<Real, Low, 4, k128, WIDE>, k128);
-    else go_up(lora_up_kernel<Real, Low, 8, 1, WIDE>, lora_up_kernel<Real, Low, 8, k256, WIDE>, k256);
+    constexpr int k128 = sizeof(Real) == 4 ? 4 : 2, k256 = k128 / 2;            // rows in LDS, by ranks
+    constexpr int kWide = sizeof(Real) == 4 ? 4 : 2;                            // tiles of outputs to a wavefront: 256 bytes of a row
+    if (pl.ranks == 32) go_up(lora_up_kernel<Real, Low, 1, 1, 2, WIDE>, lora_up_kernel<Real, Low, 1, 4, kWide, WIDE>, 4);
+    else if (pl.ranks == 64) go_up(lora_up_kernel<Real, Low, 2, 1, 2, WIDE>, lora_up_kernel<Real, Low, 2, 4, kWide, WIDE>, 4);
+    else if (pl.ranks == 128) go_up(lora_up_kernel<Real, Low, 4, 1, 2, WIDE>, lora_up_kernel<Real, Low, 4, k128, kWide, WIDE>, k128);
+    else go_up(lora_up_kernel<Real, Low, 8, 1, 2, WIDE>, lora_up_kernel<Real, Low, 8, k256, 2, WIDE>, k256);
 }
 
 }  // namespace
@@ -363,7 +475,7 @@ int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out,
     const LoraPlan pl(T, n_in, n_out, N, R, real);
     if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_lora_rows: workspace too small");
     uint8_t *ws = (uint8_t *)workspace;
-    const LoraArgs p{T, n_in, n_out, N, R, x, x_stride, a, b, adapter, scale, base, base_stride, out, out_stride, pl.slices, pl.steps, pl.range, pl.ranks,
+    const LoraArgs p{T, n_in, n_out, N, R, x, x_stride, a, b, adapter, scale, base, base_stride, out, out_stride, pl.slices, pl.steps, pl.range, pl.chunks, pl.ranks,
                      ws, pl.direct ? nullptr : (int32_t *)(ws + pl.h_bytes), (Tile *)(ws + pl.h_bytes + pl.order_bytes)};
     const size_t er = type_bytes(real), el = type_bytes(low);
     auto fits = [](const void *at, int64_t elements, size_t size) { return ((uintptr_t)at | (uintptr_t)(elements * size)) % 16 == 0; };
