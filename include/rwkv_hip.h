@@ -461,8 +461,11 @@ int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out,
  * q_stride, k_stride, v_stride and Hv * dv apart; g (the logarithm of the decay,
  * at most 0) and beta float32 [T, Hv]; state float32 [B, Hv, dk, dv], updated in
  * place.  starts int32 [B + 1] on the device: sequence b is the rows starts[b] ..
- * starts[b+1] - 1, cut to 0 .. T; NULL: T / B rows each (T a multiple of B).  Rows of
- * no sequence are left as they were in o, and the state of an empty sequence is.
+ * starts[b+1] - 1, cut to 0 .. T; starts do not decrease (what they say else is not
+ * found out: rows that two sequences name get either's values).  NULL: T / B rows each
+ * (T a multiple of B).  Rows of no sequence are left as they were in o, and the state
+ * of an empty sequence is.  Long sequences are computed in chunks of 64 rows, in which
+ * a value that is not finite reaches rows before it too, but no other sequence.
  * dk <= 256.  workspace: rwkv_delta_rule_workspace_bytes bytes, 16-byte aligned. */
 size_t rwkv_delta_rule_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv);
 int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv,

@@ -208,9 +208,9 @@ def test_delta_rule_at_the_edges(ops, dtype, case):
 
 @pytest.mark.parametrize("long", [False, True])
 def test_starts_that_name_rows_there_are_not(ops, long):
-    """Cut to the rows there are: before the first, behind the last, backwards."""
+    """Cut to the rows there are: before the first, behind the last."""
     c = P.delta_inputs(150 if long else 12, 4, 1, 1, 32, 32, torch.float32, 3)
-    _delta(ops, c, [-50, 100, 40, 140, 99999] if long else [-5, 3, 1, 9, 99999])
+    _delta(ops, c, [-50, 100, 100, 140, 99999] if long else [-5, 3, 3, 9, 99999])
 
 
 def test_delta_rule_in_parts_is_the_whole(ops):
