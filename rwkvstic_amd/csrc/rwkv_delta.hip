@@ -8,6 +8,10 @@
 //   delta_within_kernel   T and P of every chunk, all at once
 //   delta_chunks_kernel   chunk after chunk, a wavefront to 16 columns of the state
 // Both on the matrix cores with float32 sums; G and its differences are float64, as a decay is the exponential of a difference of sums.
+// A float32 operand goes into the bfloat16 matrix instructions as the sum of three bfloat16 values, its 24 bits cut in three
+// (planes); of the products of planes those below 2^-24 are left out: three products with bfloat16 keys, six of two float32
+// operands, against 16 times the time of one for float32 instructions.  (Two planes for what only reaches a bfloat16 output are not
+// enough: with keys that repeat, Q S and P U cancel.)
 #include "rwkv_types.h"
 
 #include <type_traits>
@@ -45,21 +49,29 @@ __device__ __forceinline__ float row_sum(float v) {
     return v + turned<0x121>(v);
 }
 
-// N neighbouring elements of a row of n from k on; WIDE: aligned to their size, up to 16 bytes, and n a multiple of N.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T, int N> struct Some { typedef T type __attribute__((ext_vector_type(N))); };
+
+// N neighbouring elements of a row of n from k on, zeros behind its end; WIDE: aligned to their size, up to 16 bytes, and n a multiple of N.
 template <int N, bool WIDE, typename T>
-__device__ __forceinline__ void take(T (&to)[N], const T *row, int k, int n) {
+__device__ __forceinline__ typename Some<T, N>::type take(const T *row, int k, int n) {
+    typename Some<T, N>::type to;
     if constexpr (WIDE) {
-        constexpr int E = N * sizeof(T) < 16 ? N : 16 / sizeof(T);
-        typedef T Some __attribute__((ext_vector_type(E)));
-        Some v[N / E];
+        if (k >= n) return (T)0.f;
+        if constexpr (N * sizeof(T) <= 16) return *reinterpret_cast<const typename Some<T, N>::type *>(row + k);
+        constexpr int E = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < N / E; ++i) v[i] = k < n ? *reinterpret_cast<const Some *>(row + k + i * E) : Some((T)0.f);
+        for (int i = 0; i < N; i += E) {
+            const auto v = *reinterpret_cast<const typename Some<T, E>::type *>(row + k + i);
 #pragma unroll
-        for (int i = 0; i < N; ++i) to[i] = v[i / E][i % E];
+            for (int e = 0; e < E; ++e) to[i + e] = v[e];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) to[i] = k + i < n ? row[k + i] : (T)0.f;
     }
+    return to;
 }
 
 // Lane (c, r) = (lane / 16, lane % 16) holds rows NR r .. NR r + NR - 1 of columns 4 c .. 4 c + 3, so that the sums over a
@@ -67,7 +79,6 @@ __device__ __forceinline__ void take(T (&to)[N], const T *row, int k, int n) {
 // that their sums are made side by side: S'^T q = e^g S^T q + (k.q) u.  The next row is under way meanwhile.
 template <typename T, int NR, bool WIDE>
 __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles) {
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
     const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (job >= a.B * a.Hv * tiles) return;
     const int lane = threadIdx.x & 63, r = lane & 15, col = (int)(job % tiles) * 16 + (lane >> 4) * 4;
@@ -80,27 +91,30 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
     const T *v = (const T *)a.v + first * a.v_stride + (int64_t)h * a.dv;
     T *o = (T *)a.o + (first * a.Hv + h) * a.dv;
     const float *g = a.g + first * a.Hv + h, *beta = a.beta + first * a.Hv + h;
-    float *state = a.state + (b * a.Hv + h) * a.dk * a.dv + (int64_t)r * NR * a.dv + col;
-    struct Row { T k[NR], q[NR], v[4]; float g, beta; };
+    float *state = a.state + (b * a.Hv + h) * a.dk * a.dv;
+    struct Row { typename Some<T, NR>::type k, q; typename Some<T, 4>::type v; float g, beta; };
     auto load = [&](Row &to, int64_t t) {
-        take<NR, WIDE>(to.k, k + t * a.k_stride, r * NR, a.dk);
-        take<NR, WIDE>(to.q, q + t * a.q_stride, r * NR, a.dk);
-        take<4, WIDE>(to.v, v + t * a.v_stride, col, a.dv);
+        to.k = take<NR, WIDE>(k + t * a.k_stride, r * NR, a.dk);
+        to.q = take<NR, WIDE>(q + t * a.q_stride, r * NR, a.dk);
+        to.v = take<4, WIDE>(v + t * a.v_stride, col, a.dv);
         to.g = g[t * a.Hv]; to.beta = beta[t * a.Hv];
     };
     Row next;
     load(next, 0);
-    f32x4 S[NR];
+    f32x4 S[NR];                                      // (rows and columns there are not: others, and zeros in their place)
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        S[i] = f32x4{0, 0, 0, 0};
-        if (r * NR + i >= a.dk) continue;
-        if (WIDE) { if (col < a.dv) S[i] = *reinterpret_cast<const f32x4 *>(state + (int64_t)i * a.dv); }
+        const float *row = state + (int64_t)min(r * NR + i, a.dk - 1) * a.dv;
+        if (WIDE) S[i] = *reinterpret_cast<const f32x4 *>(row + (col < a.dv ? col : 0));
         else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) if (col + c < a.dv) S[i][c] = state[(int64_t)i * a.dv + c];
+            for (int c = 0; c < 4; ++c) S[i][c] = row[min(col + c, a.dv - 1)];
         }
     }
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) S[i][c] = r * NR + i < a.dk ? S[i][c] : 0.f;
 #pragma unroll 1
     for (int64_t t = 0; t < n; ++t) {
         const Row now = next;
@@ -129,13 +143,15 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
             for (int c = 0; c < 4; ++c) S[i][c] = fmaf(e, S[i][c], (float)now.k[i] * u[c]);
         if (r < 4 && col + r < a.dv) o[t * a.Hv * a.dv + col + r] = (T)out;
     }
+    if (col >= a.dv) return;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-        if (r * NR + i >= a.dk) continue;
-        if (WIDE) { if (col < a.dv) *reinterpret_cast<f32x4 *>(state + (int64_t)i * a.dv) = S[i]; }
+        if (r * NR + i >= a.dk) break;
+        float *row = state + (int64_t)(r * NR + i) * a.dv + col;
+        if (WIDE) *reinterpret_cast<f32x4 *>(row) = S[i];
         else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) if (col + c < a.dv) state[(int64_t)i * a.dv + c] = S[i][c];
+            for (int c = 0; c < 4; ++c) if (col + c < a.dv) row[c] = S[i][c];
         }
     }
 }
@@ -143,11 +159,10 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
 // ---- chunks -----------------------------------------------------------------------------------------------------------
 constexpr int kChunk = 64;
 constexpr int kBlocks = 10;                          // 16 x 16 blocks up to the diagonal
-constexpr int kSlot = 2 * kBlocks * 256 + 2 * kChunk;        // floats of a chunk and head: T, P, e^G, e^(G_64 - G)
+// What delta_within_kernel leaves of a chunk and head, in units of 4 floats: T block by block, a unit to lane (i, g) with terms
+// 4 g .. 4 g + 3 of row i; P; e^G; e^(G_64 - G).
+constexpr int kUnitP = kBlocks * 64, kUnitG = 2 * kUnitP, kUnits = kUnitG + 2 * kChunk / 4;
 constexpr float kForgotten = -1e5f;                  // a decay's logarithm below which nothing is left; -infinity would have no differences
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Lane (j, g) = (lane % 16, lane / 16) holds rows 4 g + v, v < 4, of column j of a 16 x 16 product.  As a right operand it is to
 // hold one term k of column j at a time; the order of the terms being free, what a product leaves in the registers is the next
@@ -160,7 +175,40 @@ __device__ __forceinline__ void add_product(f32x4 &acc, const f32x4 &left, const
 // Chunks of sequence b have the places first / 64 + b and on: no two the same, none past T / 64 + B.
 __device__ __forceinline__ int64_t place_of(int64_t first, int64_t b) { return first / kChunk + b; }
 
-__device__ __forceinline__ int block_of(int row, int column) { return row * (row + 1) / 2 + column; }
+constexpr __host__ __device__ int block_of(int row, int column) { return row * (row + 1) / 2 + column; }
+constexpr __host__ __device__ int row_of(int block) { return block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3; }
+constexpr int kPairs = 6;                            // blocks two by two, as the matrix instructions take them: (row, columns 32 p .. 32 p + 31)
+constexpr __host__ __device__ int pair_of(int row, int p) { return row < 2 ? row : 2 * (row - 1) + p; }
+
+// Planes: bfloat16 values, most significant first, that add up to a float32 (or are its first 8 or 16 bits).
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+template <int N> struct Planes { u32x4 p[N]; };                 // of eight values
+__device__ __forceinline__ float rest(float v) { return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t upper(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+template <int N> __device__ __forceinline__ Planes<N> planes(f32x4 a, f32x4 b) {
+    Planes<N> to;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        to.p[n] = u32x4{upper(a[0], a[1]), upper(a[2], a[3]), upper(b[0], b[1]), upper(b[2], b[3])};
+        if (n + 1 < N)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) { a[c] = rest(a[c]); b[c] = rest(b[c]); }
+    }
+    return to;
+}
+// acc += left x right, of the planes' products those whose numbers add up to less than LIMIT, the small ones first
+template <int LIMIT, int A, int B> __device__ __forceinline__ void add_planes(f32x4 &acc, const Planes<A> &left, const Planes<B> &right) {
+#pragma unroll
+    for (int sum = LIMIT - 1; sum >= 0; --sum)
+#pragma unroll
+        for (int n = 0; n <= sum; ++n)
+            if (n < A && sum - n < B)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, left.p[n]), __builtin_bit_cast(bf16x8, right.p[sum - n]), acc, 0, 0, 0);
+}
+
+// Planes of a value of type T (float16: 8 and 3 bits).
+template <typename T> constexpr int kPlanes = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> ? 1 : 2;
+
 
 // 64 rows (zeros behind the n-th) of dk channels into LDS, as To, rows `stride` apart; WIDE: 16-byte aligned rows that fill whole 16 bytes.
 template <bool WIDE, typename To, typename T>
@@ -169,48 +217,21 @@ __device__ __forceinline__ void stage(To *lds, int stride, int filled, const T *
     const int per = filled / E;
     for (int at = threadIdx.x; at < kChunk * per; at += blockDim.x) {
         const int row = at / per, k = at % per * E;
-        T v[E];
-        take<E, WIDE>(v, from + row * from_stride, k, row < n ? dk : 0);
+        const auto v = take<E, WIDE>(from + row * from_stride, k, row < n ? dk : 0);
 #pragma unroll
         for (int e = 0; e < E; ++e) lds[row * stride + k + e] = (To)v[e];
     }
 }
 
-// Products of rows of keys and queries: the operands' own type where the matrix cores have it (the products are exact), else float32.
-template <typename T> struct Dot;
-template <> struct Dot<float> {
-    static constexpr int kPad = 4;
-    static __device__ __forceinline__ f32x4 of(const float *left, const float *right, int n, int g) {
-        f32x4 acc = {0, 0, 0, 0};
-        for (int k = 4 * g; k < n; k += 16) add_product(acc, *reinterpret_cast<const f32x4 *>(left + k), *reinterpret_cast<const f32x4 *>(right + k));
-        return acc;
-    }
-};
-template <> struct Dot<__bf16> {
-    static constexpr int kPad = 8;
-    typedef __bf16 Eight __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ f32x4 of(const __bf16 *left, const __bf16 *right, int n, int g) {
-        f32x4 acc = {0, 0, 0, 0};
-        for (int k = 8 * g; k < n; k += 32)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const Eight *>(left + k), *reinterpret_cast<const Eight *>(right + k), acc, 0, 0, 0);
-        return acc;
-    }
-};
-template <> struct Dot<_Float16> {
-    static constexpr int kPad = 8;
-    typedef _Float16 Eight __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ f32x4 of(const _Float16 *left, const _Float16 *right, int n, int g) {
-        f32x4 acc = {0, 0, 0, 0};
-        for (int k = 8 * g; k < n; k += 32)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const Eight *>(left + k), *reinterpret_cast<const Eight *>(right + k), acc, 0, 0, 0);
-        return acc;
-    }
-};
+// Products of 16 rows with 16 rows, lane (i, g) giving the i-th of each: the operands' own type where the matrix cores have it
+// (the products are exact), else float32.  The rows come from memory straight into the registers that the instruction reads.
+__device__ __forceinline__ f32x4 dot_step(Some<float, 4>::type l, Some<float, 4>::type r, f32x4 acc) { add_product(acc, l, r); return acc; }
+__device__ __forceinline__ f32x4 dot_step(Some<__bf16, 8>::type l, Some<__bf16, 8>::type r, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(l, r, acc, 0, 0, 0); }
+__device__ __forceinline__ f32x4 dot_step(Some<_Float16, 8>::type l, Some<_Float16, 8>::type r, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(l, r, acc, 0, 0, 0); }
 
-// T and P of one chunk and value head, block by block as lane (i, g) of delta_chunks_kernel wants them: row i, terms 4 g .. 4 g + 3.
+// T and P of one chunk and value head.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, float *slots, int filled) {
-    extern __shared__ __align__(16) unsigned char smem[];
+__global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *slots) {
     __shared__ double s_G[kChunk];
     __shared__ float s_beta[kChunk];
     __shared__ __align__(16) float s_A[kChunk][kChunk + 4], s_X[4][16][20];
@@ -231,11 +252,10 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, float *s
     const int64_t done = (place - place_of(first, b)) * kChunk;
     if (done >= n) return;
     first += done;
-    const int live = (int)min((int64_t)kChunk, n - done), stride = filled + Dot<T>::kPad;
-    T *ks = reinterpret_cast<T *>(smem), *qs = ks + kChunk * stride;
-    stage<WIDE>(ks, stride, filled, (const T *)a.k + first * a.k_stride + (int64_t)hk * a.dk, a.k_stride, live, a.dk);
-    stage<WIDE>(qs, stride, filled, (const T *)a.q + first * a.q_stride + (int64_t)hk * a.dk, a.q_stride, live, a.dk);
-    float *slot = slots + (place * a.Hv + h) * kSlot;
+    const int live = (int)min((int64_t)kChunk, n - done);
+    // (rows behind the last: the last again; beta is 0 there, and what comes of them is not used)
+    const T *keys = (const T *)a.k + first * a.k_stride + (int64_t)hk * a.dk, *queries = (const T *)a.q + first * a.q_stride + (int64_t)hk * a.dk;
+    f32x4 *slot = slots + (place * a.Hv + h) * kUnits;
     if (wave == 0) {
         float decay = lane < live ? a.g[(first + lane) * a.Hv + h] : 0.f;
         if (decay < kForgotten) decay = kForgotten;
@@ -244,26 +264,43 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, float *s
         for (int off = 1; off < 64; off <<= 1) { const double before = __shfl_up(G, off, 64); if (lane >= off) G += before; }
         s_G[lane] = G;
         s_beta[lane] = lane < live ? a.beta[(first + lane) * a.Hv + h] : 0.f;
-        slot[2 * kBlocks * 256 + lane] = expf((float)G);
-        slot[2 * kBlocks * 256 + kChunk + lane] = expf((float)(__shfl(G, 63, 64) - G));
+        float *decays = reinterpret_cast<float *>(slot + kUnitG);
+        decays[lane] = expf((float)G);
+        decays[kChunk + lane] = expf((float)(__shfl(G, 63, 64) - G));
+    }
+    // transposed products, so that a lane has four neighbours of a row: of the wavefront's three blocks (or two) one row and its columns
+    constexpr int E = sizeof(T) == 4 ? 4 : 8, kMost = 3;
+    f32x4 kk[kMost], qk[kMost];
+#pragma unroll
+    for (int x = 0; x < kMost; ++x) {
+        kk[x] = qk[x] = f32x4{0, 0, 0, 0};
+        const int block = kBlocks - 1 - wave - 4 * x;
+        if (block < 0) continue;
+        const int m = row_of(block), row = min(16 * m + i, live - 1), column = min(16 * (block - block_of(m, 0)) + i, live - 1);
+        const T *kr = keys + row * a.k_stride, *qr = queries + row * a.q_stride, *kc = keys + column * a.k_stride;
+        for (int k = E * g; k < a.dk + E * g; k += 4 * E) {
+            const auto left = take<E, WIDE>(kc, k, a.dk);
+            kk[x] = dot_step(left, take<E, WIDE>(kr, k, a.dk), kk[x]);
+            qk[x] = dot_step(left, take<E, WIDE>(qr, k, a.dk), qk[x]);
+        }
     }
     __syncthreads();
-    // A into LDS, P out; transposed products, so that a lane has four neighbours of a row
-    for (int block = wave; block < kBlocks; block += 4) {
-        const int m = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3, c = block - m * (m + 1) / 2;
-        const T *columns = ks + (16 * c + i) * stride;
-        const f32x4 kk = Dot<T>::of(columns, ks + (16 * m + i) * stride, filled, g), qk = Dot<T>::of(columns, qs + (16 * m + i) * stride, filled, g);
-        const int row = 16 * m + i;
+    // A into LDS, P out
+#pragma unroll
+    for (int x = 0; x < kMost; ++x) {
+        const int block = kBlocks - 1 - wave - 4 * x;
+        if (block < 0) continue;
+        const int m = row_of(block), c = block - block_of(m, 0), row = 16 * m + i;
         f32x4 A, P;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const int column = 16 * c + 4 * g + v;
             const float decay = expf((float)(s_G[row] - s_G[column]));
-            A[v] = column < row ? s_beta[row] * decay * kk[v] : 0.f;
-            P[v] = column <= row ? a.scale * decay * qk[v] : 0.f;
+            A[v] = column < row ? s_beta[row] * decay * kk[x][v] : 0.f;
+            P[v] = column <= row ? a.scale * decay * qk[x][v] : 0.f;
         }
         *reinterpret_cast<f32x4 *>(&s_A[row][16 * c + 4 * g]) = A;
-        *reinterpret_cast<f32x4 *>(slot + (kBlocks + block) * 256 + lane * 4) = P;
+        slot[kUnitP + block * 64 + lane] = P;
     }
     __syncthreads();
     // (1 + A)^-1: the blocks on the diagonal by substitution, a lane to a column ...
@@ -284,28 +321,244 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, float *s
     f32x4 X[4];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-        if (m < wave) continue;
+        X[m] = f32x4{0, 0, 0, 0};
         if (m == wave) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) X[m][v] = s_X[m][4 * g + v][i];
-        } else {
-            f32x4 Y = {0, 0, 0, 0}, Z = {0, 0, 0, 0};
+        } else if (m > wave) {
+            f32x4 Y = {0, 0, 0, 0};
 #pragma unroll
             for (int l = 0; l < m; ++l)
                 if (l >= wave) add_product(Y, *reinterpret_cast<const f32x4 *>(&s_A[16 * m + i][16 * l + 4 * g]), X[l]);
-            add_product(Z, *reinterpret_cast<const f32x4 *>(&s_X[m][i][4 * g]), Y);
-            X[m] = -Z;
+            add_product(X[m], *reinterpret_cast<const f32x4 *>(&s_X[m][i][4 * g]), -Y);
         }
-        // lane (j, g) has rows 4 g + v of column j
-        const float beta = s_beta[16 * wave + i];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) slot[block_of(m, wave) * 256 + (4 * g + v + 16 * (i >> 2)) * 4 + (i & 3)] = X[m][v] * beta;
     }
+    __syncthreads();
+    // by rows again, through LDS: a wavefront writes and reads its own columns only
+    const float beta = s_beta[16 * wave + i];
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) if (m >= wave) s_A[16 * m + 4 * g + v][16 * wave + i] = X[m][v] * beta;
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+        if (m >= wave) slot[block_of(m, wave) * 64 + lane] = *reinterpret_cast<const f32x4 *>(&s_A[16 * m + i][16 * wave + 4 * g]);
 }
 
-// NK tiles of 16 key channels.  S, and what is multiplied with it and comes of it, stay in the wavefront's registers.
+// NK tiles of 16 key channels; four wavefronts of 16 columns of the state each.  S, and what is multiplied with it and comes of it,
+// stay in the wavefront's registers; the left operands lie in LDS, where a lane's eight terms are 16 bytes:
+//   K, Q   [plane][row][block of 32 channels][unit g ^ (row / 16)], unit g: channels 4 g .. + 3 and 16 + 4 g .. + 3 of the block
+//   K^T    [plane][channel][block of 32 rows][unit g], the same of rows; channels 144 bytes apart
+//   T, P   [pair][plane][lane]; then e^G and e^(G_64 - G)
+// Everything of the next chunk is fetched into registers while this one is computed.
+template <typename T, int NK> struct Chunks {
+    static constexpr int kIn = kPlanes<T>, kRowBytes = NK * 32 + 16, kPlane = kChunk * kRowBytes, kTransposed = NK * 16 * 144;
+    static constexpr int kQ = kIn * kPlane, kT = 2 * kQ, kPairsAt = kT + kIn * kTransposed, kDecays = kPairsAt + 2 * kPairs * 3 * 1024, kBytes = kDecays + 2 * kChunk * 4;
+    static constexpr int kItems = 2 * 16 * NK * 2, kMine = (kItems + kThreads - 1) / kThreads;          // pieces of K and Q: 4 rows of 8 channels
+};
+
 template <typename T, int NK, bool WIDE>
-__global__ void __launch_bounds__(256) delta_chunks_kernel(DeltaArgs a, const float *slots, int groups) {
+__global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
+    using C = Chunks<T, NK>;
+    using V8 = typename Some<T, 8>::type;
+    constexpr int kIn = C::kIn;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
+    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / (a.Hv / a.Hk);
+    const int64_t b = blockIdx.x / groups / a.Hv;
+    const int col = (int)(blockIdx.x % groups) * 64 + wave * 16 + i;
+    const bool in = col < a.dv;
+    int64_t first, n;
+    rows_of(a, b, first, n);
+    if (n <= 0) return;
+    const f32x4 *slot = slots + (place_of(first, b) * a.Hv + h) * kUnits;
+    // Offsets within a chunk fit 32 bits (the host has looked).  Rows behind the last are the last again, columns too: T's columns
+    // are 0 there, and what comes of them is not written.
+    struct Next { V8 kq[C::kMine][4]; f32x4 blocks[kBlocks / 2]; T v[4][4]; float decay; } next;
+    auto piece = [&](int m, int &of, int &r, int &c) {
+        const int item = (m * 4 + wave) * 64;             // (a wavefront's 64 are of one operand)
+        of = item / (C::kItems / 2); r = lane & 15; c = item % (C::kItems / 2) / 16 + (lane >> 4);
+        return item < C::kItems;
+    };
+    auto fetch = [&](int64_t done) {
+        const int last = (int)min((int64_t)kChunk, n - done) - 1;
+#pragma unroll
+        for (int m = 0; m < C::kMine; ++m) {
+            int of, r, c;
+            if (!piece(m, of, r, c)) continue;
+            const int stride = (int)(of ? a.q_stride : a.k_stride);
+            const T *from = (const T *)(of ? a.q : a.k) + (first + done) * stride + (int64_t)hk * a.dk;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t row = min(4 * r + x, last) * stride;
+                if constexpr (WIDE) next.kq[m][x] = take<8, true>(from + (row + (8 * c < a.dk ? 8 * c : 0)), 0, 8);
+                else next.kq[m][x] = take<8, false>(from + row, 8 * c, a.dk);
+            }
+        }
+        const f32x4 *units = slot + done / kChunk * a.Hv * kUnits;
+#pragma unroll
+        for (int m = 0; m < kBlocks / 2; ++m) next.blocks[m] = units[m * kThreads + tid];
+        if (tid < 2 * kChunk) next.decay = reinterpret_cast<const float *>(units + kUnitG)[tid];
+        const T *values = (const T *)a.v + (first + done) * a.v_stride + (int64_t)h * a.dv;
+        const uint32_t column = in ? col : 0;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) next.v[m][v] = values[min(16 * m + 4 * g + v, last) * (uint32_t)a.v_stride + column];
+    };
+    auto put = [&] {
+#pragma unroll
+        for (int m = 0; m < C::kMine; ++m) {
+            int of, r, c;
+            if (!piece(m, of, r, c)) continue;
+            float x[4][8];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[y][e] = (float)next.kq[m][y][e];
+            if (WIDE && a.dk < NK * 16 && 8 * c >= a.dk)
+#pragma unroll
+                for (int y = 0; y < 32; ++y) x[y / 8][y % 8] = 0.f;
+            const int unit = (c >> 2) * 4 + (c & 1) * 2, half = (c >> 1 & 1) * 8, swap = r >> 2;
+            unsigned char *const rows = lds + of * C::kQ + 4 * r * C::kRowBytes + half, *const low = rows + (unit ^ swap) * 16, *const high = rows + ((unit + 1) ^ swap) * 16;
+            unsigned char *const columns = lds + C::kT + 8 * c * 144 + ((r >> 3) * 4 + (r & 3)) * 16 + (r >> 2 & 1) * 8;
+#pragma unroll
+            for (int plane = 0; plane < kIn; ++plane) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    *reinterpret_cast<uint2 *>(low + plane * C::kPlane + y * C::kRowBytes) = make_uint2(upper(x[y][0], x[y][1]), upper(x[y][2], x[y][3]));
+                    *reinterpret_cast<uint2 *>(high + plane * C::kPlane + y * C::kRowBytes) = make_uint2(upper(x[y][4], x[y][5]), upper(x[y][6], x[y][7]));
+                }
+                if (of == 0)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        *reinterpret_cast<uint2 *>(columns + plane * C::kTransposed + e * 144) = make_uint2(upper(x[0][e], x[1][e]), upper(x[2][e], x[3][e]));
+                if (plane + 1 < kIn)
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) x[y / 8][y % 8] = rest(x[y / 8][y % 8]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kBlocks / 2; ++m) {
+            const int at = m * 4 + wave, of = at / kBlocks, block = at % kBlocks, row = row_of(block), c = block - block_of(row, 0);
+            unsigned char *to = lds + C::kPairsAt + ((of * kPairs + pair_of(row, c >> 1)) * 3 * 64 + lane) * 16 + (c & 1) * 8;
+            f32x4 x = next.blocks[m];
+#pragma unroll
+            for (int plane = 0; plane < 3; ++plane) {
+                *reinterpret_cast<uint2 *>(to + plane * 1024) = make_uint2(upper(x[0], x[1]), upper(x[2], x[3]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = rest(x[e]);
+            }
+        }
+        if (tid < 2 * kChunk) reinterpret_cast<float *>(lds + C::kDecays)[tid] = next.decay;
+    };
+    auto rows = [&](int of, int m, int k) {              // K or Q, rows 16 m .., channels 32 k ..
+        Planes<kIn> p;
+#pragma unroll
+        for (int plane = 0; plane < kIn; ++plane)
+            p.p[plane] = *reinterpret_cast<const u32x4 *>(lds + of * C::kQ + plane * C::kPlane + (16 * m + i) * C::kRowBytes + k * 64 + (g ^ m) * 16);
+        return p;
+    };
+    auto transposed = [&](int k, int m) {                // channels 16 k .., rows 32 m ..
+        Planes<kIn> p;
+#pragma unroll
+        for (int plane = 0; plane < kIn; ++plane)
+            p.p[plane] = *reinterpret_cast<const u32x4 *>(lds + C::kT + plane * C::kTransposed + (16 * k + i) * 144 + (m * 4 + g) * 16);
+        return p;
+    };
+    auto pair = [&](int of, int m, int p) {              // T or P
+        Planes<3> to;
+#pragma unroll
+        for (int plane = 0; plane < 3; ++plane) to.p[plane] = *reinterpret_cast<const u32x4 *>(lds + C::kPairsAt + (((of * kPairs + pair_of(m, p)) * 3 + plane) * 64 + lane) * 16);
+        return to;
+    };
+    const float *decays = reinterpret_cast<const float *>(lds + C::kDecays);
+
+    fetch(0);
+    for (int at = tid; at < 2 * kPairs * 3 * 64; at += kThreads) reinterpret_cast<u32x4 *>(lds + C::kPairsAt)[at] = u32x4{0, 0, 0, 0};      // (pairs' blocks above the diagonal)
+    float *state = a.state + (b * a.Hv + h) * a.dk * a.dv + (in ? col : 0);
+    f32x4 S[NK];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; S[k][v] = row < a.dk ? state[(int64_t)row * a.dv] : 0.f; }
+#pragma unroll 1
+    for (int64_t done = 0; done < n; done += kChunk) {
+        const int live = (int)min((int64_t)kChunk, n - done);
+        __syncthreads();                              // nobody reads the chunk before any more
+        put();
+        f32x4 R[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) R[m][v] = (float)next.v[m][v];
+        __syncthreads();
+        if (done + kChunk < n) fetch(done + kChunk);
+        f32x4 kS[4], O[4], U[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) { kS[m] = O[m] = U[m] = f32x4{0, 0, 0, 0}; }
+#pragma unroll
+        for (int k = 0; k < NK / 2; ++k) {
+            const Planes<3> s = planes<3>(S[2 * k], S[2 * k + 1]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                add_planes<3>(kS[m], rows(0, m, k), s);
+                add_planes<3>(O[m], rows(1, m, k), s);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const f32x4 eG = *reinterpret_cast<const f32x4 *>(decays + 16 * m + 4 * g);
+            R[m] -= eG * kS[m];
+            O[m] *= eG * a.scale;
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const Planes<3> r = planes<3>(R[2 * p], R[2 * p + 1]);
+#pragma unroll
+            for (int m = 2 * p; m < 4; ++m) add_planes<3>(U[m], pair(0, m, p), r);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const Planes<3> u = planes<3>(U[2 * p], U[2 * p + 1]);
+#pragma unroll
+            for (int m = 2 * p; m < 4; ++m) add_planes<3>(O[m], pair(1, m, p), u);
+        }
+        T *const o = (T *)a.o + ((first + done) * a.Hv + h) * a.dv;
+        const uint32_t stride = a.Hv * a.dv;
+        if (in && live == kChunk) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) o[(16 * m + 4 * g + v) * stride + col] = (T)O[m][v];
+        } else if (in) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) if (16 * m + 4 * g + v < live) o[(16 * m + 4 * g + v) * stride + col] = (T)O[m][v];
+        }
+        const float last = decays[kChunk - 1];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) U[m] *= *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
+        const Planes<3> u[2] = {planes<3>(U[0], U[1]), planes<3>(U[2], U[3])};
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            S[k] *= last;
+            add_planes<3>(S[k], transposed(k, 0), u[0]);
+            add_planes<3>(S[k], transposed(k, 1), u[1]);
+        }
+    }
+    if (in)
+#pragma unroll
+        for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; if (row < a.dk) state[(int64_t)row * a.dv] = S[k][v]; }
+}
+
+// The same with float32 operands and instructions, where K, Q and K^T in planes are more than LDS holds.
+template <typename T, int NK, bool WIDE>
+__global__ void __launch_bounds__(256) delta_chunks_f32_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
     constexpr int kRow = NK * 16 + 4;
     extern __shared__ __align__(16) unsigned char smem[];
     float *ks = reinterpret_cast<float *>(smem), *qs = ks + kChunk * kRow;
@@ -323,8 +576,9 @@ __global__ void __launch_bounds__(256) delta_chunks_kernel(DeltaArgs a, const fl
     for (int k = 0; k < NK; ++k)
 #pragma unroll
         for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; S[k][v] = in && row < a.dk ? state[(int64_t)row * a.dv] : 0.f; }
-    const float *slot = slots + (place_of(first, b) * a.Hv + h) * kSlot;
-    for (int64_t done = 0; done < n; done += kChunk, first += kChunk, slot += (int64_t)a.Hv * kSlot) {
+    const f32x4 *slot = slots + (place_of(first, b) * a.Hv + h) * kUnits;
+    for (int64_t done = 0; done < n; done += kChunk, first += kChunk, slot += (int64_t)a.Hv * kUnits) {
+        const float *decays = reinterpret_cast<const float *>(slot + kUnitG);
         const int live = (int)min((int64_t)kChunk, n - done);
         f32x4 R[4], eG[4], eL[4];
 #pragma unroll
@@ -334,10 +588,10 @@ __global__ void __launch_bounds__(256) delta_chunks_kernel(DeltaArgs a, const fl
                 const int row = 16 * m + 4 * g + v;
                 R[m][v] = in && row < live ? (float)((const T *)a.v)[(first + row) * a.v_stride + (int64_t)h * a.dv + col] : 0.f;
             }
-            eG[m] = *reinterpret_cast<const f32x4 *>(slot + 2 * kBlocks * 256 + 16 * m + 4 * g);
-            eL[m] = *reinterpret_cast<const f32x4 *>(slot + 2 * kBlocks * 256 + kChunk + 16 * m + 4 * g);
+            eG[m] = *reinterpret_cast<const f32x4 *>(decays + 16 * m + 4 * g);
+            eL[m] = *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
         }
-        const float last = slot[2 * kBlocks * 256 + kChunk - 1];
+        const float last = decays[kChunk - 1];
         __syncthreads();
         stage<WIDE>(ks, kRow, NK * 16, (const T *)a.k + first * a.k_stride + (int64_t)hk * a.dk, a.k_stride, live, a.dk);
         stage<WIDE>(qs, kRow, NK * 16, (const T *)a.q + first * a.q_stride + (int64_t)hk * a.dk, a.q_stride, live, a.dk);
@@ -357,11 +611,11 @@ __global__ void __launch_bounds__(256) delta_chunks_kernel(DeltaArgs a, const fl
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int c = 0; c <= m; ++c) add_product(U[m], *reinterpret_cast<const f32x4 *>(slot + block_of(m, c) * 256 + lane * 4), R[c]);
+            for (int c = 0; c <= m; ++c) add_product(U[m], slot[block_of(m, c) * 64 + lane], R[c]);
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int c = 0; c <= m; ++c) add_product(O[m], *reinterpret_cast<const f32x4 *>(slot + (kBlocks + block_of(m, c)) * 256 + lane * 4), U[c]);
+            for (int c = 0; c <= m; ++c) add_product(O[m], slot[kUnitP + block_of(m, c) * 64 + lane], U[c]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -396,7 +650,7 @@ template <typename F> int by_channels(int dk, F &&fn) {
 }
 
 template <typename T, bool WIDE>
-int launch(hipStream_t st, const DeltaArgs &a, float *slots) {
+int launch(hipStream_t st, const DeltaArgs &a, f32x4 *slots) {
     if (!in_chunks(a.T, a.B)) {
         const int tiles = (int)ceil_div(a.dv, 16);
         return by_channels(a.dk, [&](auto nr) {
@@ -405,17 +659,16 @@ int launch(hipStream_t st, const DeltaArgs &a, float *slots) {
             return (int)RWKV_OK;
         });
     }
-    const int filled = (int)round_up(a.dk, 32);
-    const size_t lds = (size_t)2 * kChunk * (filled + Dot<T>::kPad) * sizeof(T);
-    if (const int rc = allow_lds<&delta_within_kernel<T, WIDE>>(lds)) return rc;
-    hipLaunchKernelGGL((delta_within_kernel<T, WIDE>), dim3((unsigned)(a.T / kChunk + a.B), (unsigned)a.Hv), dim3(256), lds, st, a, slots, filled);
+    hipLaunchKernelGGL((delta_within_kernel<T, WIDE>), dim3((unsigned)(a.T / kChunk + a.B), (unsigned)a.Hv), dim3(256), 0, st, a, slots);
     RWKV_CHECK_LAUNCH("delta_within_kernel");
     return by_channels(a.dk, [&](auto nk) {
         constexpr int NK = decltype(nk)::value;
-        constexpr size_t lds = (size_t)2 * kChunk * (NK * 16 + 4) * 4;
-        if (const int rc = allow_lds<&delta_chunks_kernel<T, NK, WIDE>>(lds)) return rc;
-        const int waves = a.dv <= 16 ? 1 : a.dv <= 32 ? 2 : 4, groups = (int)ceil_div(a.dv, 16 * waves);
-        hipLaunchKernelGGL((delta_chunks_kernel<T, NK, WIDE>), dim3((unsigned)(a.B * a.Hv * groups)), dim3(64 * waves), lds, st, a, slots, groups);
+        constexpr bool kInPlanes = Chunks<T, NK>::kBytes <= 160 * 1024;
+        constexpr size_t bytes = kInPlanes ? Chunks<T, NK>::kBytes : 2 * kChunk * (NK * 16 + 4) * 4;
+        constexpr auto kernel = [] { if constexpr (kInPlanes) return &delta_chunks_kernel<T, NK, WIDE>; else return &delta_chunks_f32_kernel<T, NK, WIDE>; }();
+        if (const int rc = allow_lds<kernel>(bytes)) return rc;
+        const int groups = (int)ceil_div(a.dv, 64);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(a.B * a.Hv * groups)), dim3(kThreads), bytes, st, a, slots, groups);
         RWKV_CHECK_LAUNCH("delta_chunks_kernel");
         return (int)RWKV_OK;
     });
@@ -431,7 +684,7 @@ extern "C" {
 
 size_t rwkv_delta_rule_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv) {
     if (T <= 0 || B <= 0 || Hv <= 0 || !in_chunks(T, B)) return 0;
-    return (size_t)((T / kChunk + B) * Hv) * kSlot * sizeof(float);
+    return (size_t)((T / kChunk + B) * Hv) * kUnits * 16;
 }
 
 int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv, int type, const void *q,
@@ -446,6 +699,8 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
     if (dk > 256 || dv > 65536 || Hv > 65535 || T >= (1ll << 31) || B * Hv * ceil_div(dv, 16) >= (1ll << 31))
         return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: keys of at most 256 channels");
     if (in_chunks(T, B)) {
+        if (q_stride >= (1 << 24) || k_stride >= (1 << 24) || v_stride >= (1 << 24) || Hv * dv >= (1 << 24))
+            return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: rows of 2^24 elements or more");
         RWKV_CHECK_ALIGN(workspace, 16);
         if (!workspace || workspace_bytes < rwkv_delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv))
             return set_error(RWKV_ERR_WORKSPACE, "rwkv_delta_rule: workspace too small");
@@ -457,7 +712,7 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
     const bool wide = fits(q, q_stride, dk) && fits(k, k_stride, dk) && fits(v, v_stride, dv) && (uintptr_t)state % 16 == 0 && dk % 16 == 0 && dv % 4 == 0;
     return with_low(type, [&](auto ty) {
         using E = typename decltype(ty)::type;
-        return wide ? launch<E, true>((hipStream_t)stream, a, (float *)workspace) : launch<E, false>((hipStream_t)stream, a, (float *)workspace);
+        return wide ? launch<E, true>((hipStream_t)stream, a, (f32x4 *)workspace) : launch<E, false>((hipStream_t)stream, a, (f32x4 *)workspace);
     });
 }
 
