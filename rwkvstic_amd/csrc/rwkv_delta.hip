@@ -196,18 +196,28 @@ template <int N> __device__ __forceinline__ Planes<N> planes(f32x4 a, f32x4 b) {
     }
     return to;
 }
-// acc += left x right, of the planes' products those whose numbers add up to less than LIMIT, the small ones first
-template <int LIMIT, int A, int B> __device__ __forceinline__ void add_planes(f32x4 &acc, const Planes<A> &left, const Planes<B> &right) {
+// acc[m] += left[m] x right, of the planes' products those whose numbers add up to less than 3, the small ones first; products of
+// different sums one after the other, as the next one of the same sum has to wait for it.  SWAPPED: the transposed product, of the same
+// registers: lane (j, g) gets columns 4 g + v of row j.
+template <bool SWAPPED = false, int M, int A, int B> __device__ __forceinline__ void add_planes(f32x4 (&acc)[M], const Planes<A> (&left)[M], const Planes<B> &right) {
 #pragma unroll
-    for (int sum = LIMIT - 1; sum >= 0; --sum)
+    for (int sum = 2; sum >= 0; --sum)
 #pragma unroll
         for (int n = 0; n <= sum; ++n)
             if (n < A && sum - n < B)
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, left.p[n]), __builtin_bit_cast(bf16x8, right.p[sum - n]), acc, 0, 0, 0);
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    const bf16x8 l = __builtin_bit_cast(bf16x8, left[m].p[n]), r = __builtin_bit_cast(bf16x8, right.p[sum - n]);
+                    acc[m] = SWAPPED ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(r, l, acc[m], 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x32_bf16(l, r, acc[m], 0, 0, 0);
+                }
 }
 
 // Planes of a value of type T (float16: 8 and 3 bits).
 template <typename T> constexpr int kPlanes = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> ? 1 : 2;
+__device__ __forceinline__ Planes<1> planes_of(bf16x8 v) { return {{__builtin_bit_cast(u32x4, v)}}; }
+template <typename V> __device__ __forceinline__ auto planes_of(V v) {
+    return planes<kPlanes<std::decay_t<decltype(v[0])>>>(f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}, f32x4{(float)v[4], (float)v[5], (float)v[6], (float)v[7]});
+}
 
 
 // 64 rows (zeros behind the n-th) of dk channels into LDS, as To, rows `stride` apart; WIDE: 16-byte aligned rows that fill whole 16 bytes.
@@ -271,18 +281,21 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
     // transposed products, so that a lane has four neighbours of a row: of the wavefront's three blocks (or two) one row and its columns
     constexpr int E = sizeof(T) == 4 ? 4 : 8, kMost = 3;
     f32x4 kk[kMost], qk[kMost];
+    const T *kr[kMost], *qr[kMost], *kc[kMost];
 #pragma unroll
     for (int x = 0; x < kMost; ++x) {
         kk[x] = qk[x] = f32x4{0, 0, 0, 0};
-        const int block = kBlocks - 1 - wave - 4 * x;
-        if (block < 0) continue;
-        const int m = row_of(block), row = min(16 * m + i, live - 1), column = min(16 * (block - block_of(m, 0)) + i, live - 1);
-        const T *kr = keys + row * a.k_stride, *qr = queries + row * a.q_stride, *kc = keys + column * a.k_stride;
-        for (int k = E * g; k < a.dk + E * g; k += 4 * E) {
-            const auto left = take<E, WIDE>(kc, k, a.dk);
-            kk[x] = dot_step(left, take<E, WIDE>(kr, k, a.dk), kk[x]);
-            qk[x] = dot_step(left, take<E, WIDE>(qr, k, a.dk), qk[x]);
-        }
+        const int block = max(kBlocks - 1 - wave - 4 * x, 0), m = row_of(block);
+        const int row = min(16 * m + i, live - 1), column = min(16 * (block - block_of(m, 0)) + i, live - 1);
+        kr[x] = keys + row * a.k_stride; qr[x] = queries + row * a.q_stride; kc[x] = keys + column * a.k_stride;
+    }
+#pragma unroll 2
+    for (int k = E * g; k < a.dk + E * g; k += 4 * E) {
+        typename Some<T, E>::type l[kMost], r[kMost], q[kMost];
+#pragma unroll
+        for (int x = 0; x < kMost; ++x) { l[x] = take<E, WIDE>(kc[x], k, a.dk); r[x] = take<E, WIDE>(kr[x], k, a.dk); q[x] = take<E, WIDE>(qr[x], k, a.dk); }
+#pragma unroll
+        for (int x = 0; x < kMost; ++x) { kk[x] = dot_step(l[x], r[x], kk[x]); qk[x] = dot_step(l[x], q[x], qk[x]); }
     }
     __syncthreads();
     // A into LDS, P out
@@ -351,11 +364,13 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
 //   K, Q   [plane][row][block of 32 channels][unit g ^ (row / 16)], unit g: channels 4 g .. + 3 and 16 + 4 g .. + 3 of the block
 //   K^T    [plane][channel][block of 32 rows][unit g], the same of rows; channels 144 bytes apart
 //   T, P   [pair][plane][lane]; then e^G and e^(G_64 - G)
+//   V^T    [column][row], columns 64 rows and 16 bytes apart
 // Everything of the next chunk is fetched into registers while this one is computed.
 template <typename T, int NK> struct Chunks {
     static constexpr int kIn = kPlanes<T>, kRowBytes = NK * 32 + 16, kPlane = kChunk * kRowBytes, kTransposed = NK * 16 * 144;
-    static constexpr int kQ = kIn * kPlane, kT = 2 * kQ, kPairsAt = kT + kIn * kTransposed, kDecays = kPairsAt + 2 * kPairs * 3 * 1024, kBytes = kDecays + 2 * kChunk * 4;
-    static constexpr int kItems = 2 * 16 * NK * 2, kMine = (kItems + kThreads - 1) / kThreads;          // pieces of K and Q: 4 rows of 8 channels
+    static constexpr int kQ = kIn * kPlane, kT = 2 * kQ, kPairsAt = kT + kIn * kTransposed, kDecays = kPairsAt + 2 * kPairs * 3 * 1024, kV = kDecays + 2 * kChunk * 4;
+    static constexpr int kColumn = kChunk * sizeof(T) + 16, kBytes = kV + 64 * kColumn;
+    static constexpr int kOf = 16 * NK * 2, kItems = 2 * kOf + 16 * 8, kMine = (kItems + kThreads - 1) / kThreads;          // pieces of K, Q and V: 4 rows of 8 channels
 };
 
 template <typename T, int NK, bool WIDE>
@@ -367,7 +382,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
     const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / (a.Hv / a.Hk);
     const int64_t b = blockIdx.x / groups / a.Hv;
-    const int col = (int)(blockIdx.x % groups) * 64 + wave * 16 + i;
+    const int col0 = (int)(blockIdx.x % groups) * 64, col = col0 + wave * 16 + i;
     const bool in = col < a.dv;
     int64_t first, n;
     rows_of(a, b, first, n);
@@ -375,10 +390,10 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     const f32x4 *slot = slots + (place_of(first, b) * a.Hv + h) * kUnits;
     // Offsets within a chunk fit 32 bits (the host has looked).  Rows behind the last are the last again, columns too: T's columns
     // are 0 there, and what comes of them is not written.
-    struct Next { V8 kq[C::kMine][4]; f32x4 blocks[kBlocks / 2]; T v[4][4]; float decay; } next;
+    struct Next { V8 rows[C::kMine][4]; f32x4 blocks[kBlocks / 2]; float decay; } next;
     auto piece = [&](int m, int &of, int &r, int &c) {
         const int item = (m * 4 + wave) * 64;             // (a wavefront's 64 are of one operand)
-        of = item / (C::kItems / 2); r = lane & 15; c = item % (C::kItems / 2) / 16 + (lane >> 4);
+        of = item / C::kOf < 2 ? item / C::kOf : 2; r = lane & 15; c = (item - of * C::kOf) / 16 + (lane >> 4);
         return item < C::kItems;
     };
     auto fetch = [&](int64_t done) {
@@ -387,56 +402,58 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
         for (int m = 0; m < C::kMine; ++m) {
             int of, r, c;
             if (!piece(m, of, r, c)) continue;
-            const int stride = (int)(of ? a.q_stride : a.k_stride);
-            const T *from = (const T *)(of ? a.q : a.k) + (first + done) * stride + (int64_t)hk * a.dk;
+            const int stride = (int)(of == 0 ? a.k_stride : of == 1 ? a.q_stride : a.v_stride), channels = of < 2 ? a.dk : a.dv - col0;
+            const T *from = (const T *)(of == 0 ? a.k : of == 1 ? a.q : a.v) + (first + done) * stride + (of < 2 ? (int64_t)hk * a.dk : (int64_t)h * a.dv + col0);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const uint32_t row = min(4 * r + x, last) * stride;
-                if constexpr (WIDE) next.kq[m][x] = take<8, true>(from + (row + (8 * c < a.dk ? 8 * c : 0)), 0, 8);
-                else next.kq[m][x] = take<8, false>(from + row, 8 * c, a.dk);
+                if constexpr (WIDE) next.rows[m][x] = take<8, true>(from + (row + (8 * c < channels ? 8 * c : 0)), 0, 8);
+                else next.rows[m][x] = take<8, false>(from + row, 8 * c, channels);
             }
         }
         const f32x4 *units = slot + done / kChunk * a.Hv * kUnits;
 #pragma unroll
         for (int m = 0; m < kBlocks / 2; ++m) next.blocks[m] = units[m * kThreads + tid];
         if (tid < 2 * kChunk) next.decay = reinterpret_cast<const float *>(units + kUnitG)[tid];
-        const T *values = (const T *)a.v + (first + done) * a.v_stride + (int64_t)h * a.dv;
-        const uint32_t column = in ? col : 0;
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) next.v[m][v] = values[min(16 * m + 4 * g + v, last) * (uint32_t)a.v_stride + column];
     };
     auto put = [&] {
 #pragma unroll
         for (int m = 0; m < C::kMine; ++m) {
             int of, r, c;
             if (!piece(m, of, r, c)) continue;
-            float x[4][8];
+            V8 x[4];
+            if (of == 2) {
+                T *const to = reinterpret_cast<T *>(lds + C::kV + 8 * c * C::kColumn) + 4 * r;
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+                for (int e = 0; e < 8; ++e) {
+                    const typename Some<T, 4>::type column = {next.rows[m][0][e], next.rows[m][1][e], next.rows[m][2][e], next.rows[m][3][e]};
+                    *reinterpret_cast<typename Some<T, 4>::type *>(reinterpret_cast<unsigned char *>(to) + e * C::kColumn) = column;
+                }
+                continue;
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[y][e] = (float)next.kq[m][y][e];
-            if (WIDE && a.dk < NK * 16 && 8 * c >= a.dk)
-#pragma unroll
-                for (int y = 0; y < 32; ++y) x[y / 8][y % 8] = 0.f;
+            for (int y = 0; y < 4; ++y) x[y] = WIDE && 8 * c >= a.dk ? V8((T)0.f) : next.rows[m][y];
             const int unit = (c >> 2) * 4 + (c & 1) * 2, half = (c >> 1 & 1) * 8, swap = r >> 2;
             unsigned char *const rows = lds + of * C::kQ + 4 * r * C::kRowBytes + half, *const low = rows + (unit ^ swap) * 16, *const high = rows + ((unit + 1) ^ swap) * 16;
             unsigned char *const columns = lds + C::kT + 8 * c * 144 + ((r >> 3) * 4 + (r & 3)) * 16 + (r >> 2 & 1) * 8;
+            Planes<kIn> cut[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) cut[y] = planes_of(x[y]);
 #pragma unroll
             for (int plane = 0; plane < kIn; ++plane) {
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                    *reinterpret_cast<uint2 *>(low + plane * C::kPlane + y * C::kRowBytes) = make_uint2(upper(x[y][0], x[y][1]), upper(x[y][2], x[y][3]));
-                    *reinterpret_cast<uint2 *>(high + plane * C::kPlane + y * C::kRowBytes) = make_uint2(upper(x[y][4], x[y][5]), upper(x[y][6], x[y][7]));
+                    const u32x4 w = cut[y].p[plane];
+                    *reinterpret_cast<uint2 *>(low + plane * C::kPlane + y * C::kRowBytes) = make_uint2(w[0], w[1]);
+                    *reinterpret_cast<uint2 *>(high + plane * C::kPlane + y * C::kRowBytes) = make_uint2(w[2], w[3]);
                 }
                 if (of == 0)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        *reinterpret_cast<uint2 *>(columns + plane * C::kTransposed + e * 144) = make_uint2(upper(x[0][e], x[1][e]), upper(x[2][e], x[3][e]));
-                if (plane + 1 < kIn)
-#pragma unroll
-                    for (int y = 0; y < 32; ++y) x[y / 8][y % 8] = rest(x[y / 8][y % 8]);
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
+                        *reinterpret_cast<uint2 *>(columns + plane * C::kTransposed + e * 144) =
+                            make_uint2(__builtin_amdgcn_perm(cut[1].p[plane][e / 2], cut[0].p[plane][e / 2], pick), __builtin_amdgcn_perm(cut[3].p[plane][e / 2], cut[2].p[plane][e / 2], pick));
+                    }
             }
         }
 #pragma unroll
@@ -488,11 +505,6 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
         const int live = (int)min((int64_t)kChunk, n - done);
         __syncthreads();                              // nobody reads the chunk before any more
         put();
-        f32x4 R[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) R[m][v] = (float)next.v[m][v];
         __syncthreads();
         if (done + kChunk < n) fetch(done + kChunk);
         f32x4 kS[4], O[4], U[4];
@@ -501,52 +513,54 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
             const Planes<3> s = planes<3>(S[2 * k], S[2 * k + 1]);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                add_planes<3>(kS[m], rows(0, m, k), s);
-                add_planes<3>(O[m], rows(1, m, k), s);
-            }
+            const Planes<kIn> keys[4] = {rows(0, 0, k), rows(0, 1, k), rows(0, 2, k), rows(0, 3, k)}, queries[4] = {rows(1, 0, k), rows(1, 1, k), rows(1, 2, k), rows(1, 3, k)};
+            add_planes(kS, keys, s);
+            add_planes<true>(O, queries, s);
         }
+        f32x4 R[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
+            const auto v = *reinterpret_cast<const typename Some<T, 4>::type *>(lds + C::kV + (wave * 16 + i) * C::kColumn + (16 * m + 4 * g) * sizeof(T));
             const f32x4 eG = *reinterpret_cast<const f32x4 *>(decays + 16 * m + 4 * g);
-            R[m] -= eG * kS[m];
-            O[m] *= eG * a.scale;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) R[m][c] = (float)v[c] - eG[c] * kS[m][c];
+            O[m] *= decays[16 * m + i] * a.scale;
         }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const Planes<3> r = planes<3>(R[2 * p], R[2 * p + 1]);
-#pragma unroll
-            for (int m = 2 * p; m < 4; ++m) add_planes<3>(U[m], pair(0, m, p), r);
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const Planes<3> u = planes<3>(U[2 * p], U[2 * p + 1]);
-#pragma unroll
-            for (int m = 2 * p; m < 4; ++m) add_planes<3>(O[m], pair(1, m, p), u);
-        }
+        auto below = [&](auto swapped, f32x4 (&acc)[4], int of, const f32x4 (&x)[4]) {         // acc += T x, or (P x)^T
+            const Planes<3> left[4] = {pair(of, 0, 0), pair(of, 1, 0), pair(of, 2, 0), pair(of, 3, 0)};
+            add_planes<decltype(swapped)::value>(acc, left, planes<3>(x[0], x[1]));
+            const Planes<3> lower[2] = {pair(of, 2, 1), pair(of, 3, 1)};
+            f32x4 two[2] = {acc[2], acc[3]};
+            add_planes<decltype(swapped)::value>(two, lower, planes<3>(x[2], x[3]));
+            acc[2] = two[0]; acc[3] = two[1];
+        };
+        below(std::false_type{}, U, 0, R);
+        below(std::true_type{}, O, 1, U);
         T *const o = (T *)a.o + ((first + done) * a.Hv + h) * a.dv;
-        const uint32_t stride = a.Hv * a.dv;
-        if (in && live == kChunk) {
+        const int from = col0 + wave * 16 + 4 * g;
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < 4; ++m) {
+            if (16 * m + i >= live) break;
+            T *const to = o + ((16 * m + i) * (uint32_t)(a.Hv * a.dv) + from);
+            if (WIDE) { if (from < a.dv) *reinterpret_cast<typename Some<T, 4>::type *>(to) = __builtin_convertvector(O[m], typename Some<T, 4>::type); }
+            else {
 #pragma unroll
-                for (int v = 0; v < 4; ++v) o[(16 * m + 4 * g + v) * stride + col] = (T)O[m][v];
-        } else if (in) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) if (16 * m + 4 * g + v < live) o[(16 * m + 4 * g + v) * stride + col] = (T)O[m][v];
+                for (int c = 0; c < 4; ++c) if (from + c < a.dv) to[c] = (T)O[m][c];
+            }
         }
         const float last = decays[kChunk - 1];
 #pragma unroll
         for (int m = 0; m < 4; ++m) U[m] *= *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
         const Planes<3> u[2] = {planes<3>(U[0], U[1]), planes<3>(U[2], U[3])};
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            S[k] *= last;
-            add_planes<3>(S[k], transposed(k, 0), u[0]);
-            add_planes<3>(S[k], transposed(k, 1), u[1]);
+        for (int k = 0; k < NK; k += 2) {
+            f32x4 two[2] = {S[k] * last, S[k + 1] * last};
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                const Planes<kIn> left[2] = {transposed(k, m), transposed(k + 1, m)};
+                add_planes(two, left, u[m]);
+            }
+            S[k] = two[0]; S[k + 1] = two[1];
         }
     }
     if (in)
@@ -709,7 +723,7 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
     const size_t size = type_bytes(type);
     auto fits = [&](const void *at, int64_t stride, int64_t channels) { return ((uintptr_t)at | (uintptr_t)(stride * size) | (uintptr_t)(channels * size)) % 16 == 0; };
     // (heads of whole 16 bytes, which are also what a lane of delta_steps_kernel takes at a time, or multiples of it)
-    const bool wide = fits(q, q_stride, dk) && fits(k, k_stride, dk) && fits(v, v_stride, dv) && (uintptr_t)state % 16 == 0 && dk % 16 == 0 && dv % 4 == 0;
+    const bool wide = fits(q, q_stride, dk) && fits(k, k_stride, dk) && fits(v, v_stride, dv) && (uintptr_t)state % 16 == 0 && (uintptr_t)o % 16 == 0 && dk % 16 == 0 && dv % 8 == 0;
     return with_low(type, [&](auto ty) {
         using E = typename decltype(ty)::type;
         return wide ? launch<E, true>((hipStream_t)stream, a, (f32x4 *)workspace) : launch<E, false>((hipStream_t)stream, a, (f32x4 *)workspace);
