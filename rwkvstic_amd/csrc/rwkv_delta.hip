@@ -115,9 +115,13 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
     for (int i = 0; i < NR; ++i)
 #pragma unroll
         for (int c = 0; c < 4; ++c) S[i][c] = r * NR + i < a.dk ? S[i][c] : 0.f;
+    // (a row's output is stored a step later, in front of the next loads: behind them, they would be waited for together)
+    float out = 0.f;
+    auto store = [&](int64_t t) { if (r < 4 && col + r < a.dv) o[t * a.Hv * a.dv + col + r] = (T)out; };
 #pragma unroll 1
     for (int64_t t = 0; t < n; ++t) {
         const Row now = next;
+        if (t) store(t - 1);
         if (t + 1 < n) load(next, t + 1);
         const float e = expf(now.g);
         float kq = 0.f;
@@ -130,7 +134,7 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
             for (int c = 0; c < 4; ++c) { kS[c] = fmaf(kk, S[i][c], kS[c]); qS[c] = fmaf(qq, S[i][c], qS[c]); }
         }
         kq = row_sum(kq);
-        float out = 0.f, u[4];
+        float u[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             u[c] = now.beta * ((float)now.v[c] - e * row_sum(kS[c]));
@@ -141,8 +145,8 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
         for (int i = 0; i < NR; ++i)
 #pragma unroll
             for (int c = 0; c < 4; ++c) S[i][c] = fmaf(e, S[i][c], (float)now.k[i] * u[c]);
-        if (r < 4 && col + r < a.dv) o[t * a.Hv * a.dv + col + r] = (T)out;
     }
+    store(n - 1);
     if (col >= a.dv) return;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
@@ -365,19 +369,21 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
 //   K^T    [plane][channel][block of 32 rows][unit g], the same of rows; channels 144 bytes apart
 //   T, P   [pair][plane][lane]; then e^G and e^(G_64 - G)
 //   V^T    [column][row], columns 64 rows and 16 bytes apart
-// Everything of the next chunk is fetched into registers while this one is computed.
+// A wavefront has its SIMD to itself, so what fetches the next chunk and puts it into LDS stands between the products of this one,
+// each part as soon as its place is free: K, Q and V by pieces of a few rows of eight channels to a thread, T and P by blocks.
 template <typename T, int NK> struct Chunks {
     static constexpr int kIn = kPlanes<T>, kRowBytes = NK * 32 + 16, kPlane = kChunk * kRowBytes, kTransposed = NK * 16 * 144;
     static constexpr int kQ = kIn * kPlane, kT = 2 * kQ, kPairsAt = kT + kIn * kTransposed, kDecays = kPairsAt + 2 * kPairs * 3 * 1024, kV = kDecays + 2 * kChunk * 4;
     static constexpr int kColumn = kChunk * sizeof(T) + 16, kBytes = kV + 64 * kColumn;
-    static constexpr int kOf = 16 * NK * 2, kItems = 2 * kOf + 16 * 8, kMine = (kItems + kThreads - 1) / kThreads;          // pieces of K, Q and V: 4 rows of 8 channels
+    static constexpr int kRows = NK >= 8 ? 4 : 2, kPieces = NK * 2 * (kChunk / kRows) / kThreads;          // rows of a piece of K or Q, pieces of a thread
 };
 
 template <typename T, int NK, bool WIDE>
 __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
     using C = Chunks<T, NK>;
     using V8 = typename Some<T, 8>::type;
-    constexpr int kIn = C::kIn;
+    using V4 = typename Some<T, 4>::type;
+    constexpr int kIn = C::kIn, kRows = C::kRows, kPieces = C::kPieces, kAcross = kChunk / kRows;
     extern __shared__ __align__(16) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
     const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / (a.Hv / a.Hk);
@@ -387,80 +393,82 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     int64_t first, n;
     rows_of(a, b, first, n);
     if (n <= 0) return;
+    const int64_t end = (n - 1) / kChunk * kChunk;       // the last chunk
     const f32x4 *slot = slots + (place_of(first, b) * a.Hv + h) * kUnits;
-    // Offsets within a chunk fit 32 bits (the host has looked).  Rows behind the last are the last again, columns too: T's columns
-    // are 0 there, and what comes of them is not written.
-    struct Next { V8 rows[C::kMine][4]; f32x4 blocks[kBlocks / 2]; float decay; } next;
-    auto piece = [&](int m, int &of, int &r, int &c) {
-        const int item = (m * 4 + wave) * 64;             // (a wavefront's 64 are of one operand)
-        of = item / C::kOf < 2 ? item / C::kOf : 2; r = lane & 15; c = (item - of * C::kOf) / 16 + (lane >> 4);
-        return item < C::kItems;
-    };
-    auto fetch = [&](int64_t done) {
+    // Offsets within a chunk fit 32 bits (the host has looked).  Rows behind the last are the last again, columns the first: T's
+    // columns are 0 there, and what comes of them is not written.  Behind the last chunk it is fetched again.
+    auto piece = [&](V8 *to, const T *from, int64_t stride, int64_t done, int count, int r, int c, int channels) {
         const int last = (int)min((int64_t)kChunk, n - done) - 1;
+        const T *chunk = from + (first + done) * stride;
 #pragma unroll
-        for (int m = 0; m < C::kMine; ++m) {
-            int of, r, c;
-            if (!piece(m, of, r, c)) continue;
-            const int stride = (int)(of == 0 ? a.k_stride : of == 1 ? a.q_stride : a.v_stride), channels = of < 2 ? a.dk : a.dv - col0;
-            const T *from = (const T *)(of == 0 ? a.k : of == 1 ? a.q : a.v) + (first + done) * stride + (of < 2 ? (int64_t)hk * a.dk : (int64_t)h * a.dv + col0);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t row = min(4 * r + x, last) * stride;
-                if constexpr (WIDE) next.rows[m][x] = take<8, true>(from + (row + (8 * c < channels ? 8 * c : 0)), 0, 8);
-                else next.rows[m][x] = take<8, false>(from + row, 8 * c, channels);
-            }
+        for (int x = 0; x < count; ++x) {
+            const uint32_t row = min(count * r + x, last) * (uint32_t)stride;
+            if constexpr (WIDE) to[x] = take<8, true>(chunk + (row + (8 * c < channels ? 8 * c : 0)), 0, 8);
+            else to[x] = take<8, false>(chunk + row, 8 * c, channels);
         }
+    };
+    V8 keys_next[kPieces][kRows], queries_next[kPieces][kRows], keys_now[kPieces][kRows], values_next[2];
+    f32x4 blocks_next[kBlocks / 2];
+    float decay_next;
+    const int r = tid % kAcross, c0 = tid / kAcross;
+    auto fetch_rows = [&](int64_t done) {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) {
+            piece(keys_next[m], (const T *)a.k + (int64_t)hk * a.dk, a.k_stride, done, kRows, r, c0 + m * (kThreads / kAcross), a.dk);
+            piece(queries_next[m], (const T *)a.q + (int64_t)hk * a.dk, a.q_stride, done, kRows, r, c0 + m * (kThreads / kAcross), a.dk);
+        }
+    };
+    auto fetch_rest = [&](int64_t done) {
         const f32x4 *units = slot + done / kChunk * a.Hv * kUnits;
 #pragma unroll
-        for (int m = 0; m < kBlocks / 2; ++m) next.blocks[m] = units[m * kThreads + tid];
-        if (tid < 2 * kChunk) next.decay = reinterpret_cast<const float *>(units + kUnitG)[tid];
+        for (int m = 0; m < kBlocks / 2; ++m) blocks_next[m] = units[m * kThreads + tid];
+        decay_next = reinterpret_cast<const float *>(units + kUnitG)[tid % (2 * kChunk)];
+        piece(values_next, (const T *)a.v + (int64_t)h * a.dv + col0, a.v_stride, done, 2, tid & 31, tid >> 5, a.dv - col0);
     };
-    auto put = [&] {
+    auto cut = [&](const V8 &x, int c) { return planes_of(WIDE && 8 * c >= a.dk ? V8((T)0.f) : x); };
+    auto put_rows = [&](const V8 (&x)[kPieces][kRows], int of) {
 #pragma unroll
-        for (int m = 0; m < C::kMine; ++m) {
-            int of, r, c;
-            if (!piece(m, of, r, c)) continue;
-            V8 x[4];
-            if (of == 2) {
-                T *const to = reinterpret_cast<T *>(lds + C::kV + 8 * c * C::kColumn) + 4 * r;
+        for (int m = 0; m < kPieces; ++m) {
+            const int c = c0 + m * (kThreads / kAcross), unit = (c >> 2) * 4 + (c & 1) * 2, half = (c >> 1 & 1) * 8, swap = kRows * r >> 4;
+            unsigned char *const to = lds + of * C::kQ + kRows * r * C::kRowBytes + half, *const low = to + (unit ^ swap) * 16, *const high = to + ((unit + 1) ^ swap) * 16;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const typename Some<T, 4>::type column = {next.rows[m][0][e], next.rows[m][1][e], next.rows[m][2][e], next.rows[m][3][e]};
-                    *reinterpret_cast<typename Some<T, 4>::type *>(reinterpret_cast<unsigned char *>(to) + e * C::kColumn) = column;
+            for (int y = 0; y < kRows; ++y) {
+                const Planes<kIn> p = cut(x[m][y], c);
+#pragma unroll
+                for (int plane = 0; plane < kIn; ++plane) {
+                    *reinterpret_cast<uint2 *>(low + plane * C::kPlane + y * C::kRowBytes) = make_uint2(p.p[plane][0], p.p[plane][1]);
+                    *reinterpret_cast<uint2 *>(high + plane * C::kPlane + y * C::kRowBytes) = make_uint2(p.p[plane][2], p.p[plane][3]);
                 }
-                continue;
-            }
-#pragma unroll
-            for (int y = 0; y < 4; ++y) x[y] = WIDE && 8 * c >= a.dk ? V8((T)0.f) : next.rows[m][y];
-            const int unit = (c >> 2) * 4 + (c & 1) * 2, half = (c >> 1 & 1) * 8, swap = r >> 2;
-            unsigned char *const rows = lds + of * C::kQ + 4 * r * C::kRowBytes + half, *const low = rows + (unit ^ swap) * 16, *const high = rows + ((unit + 1) ^ swap) * 16;
-            unsigned char *const columns = lds + C::kT + 8 * c * 144 + ((r >> 3) * 4 + (r & 3)) * 16 + (r >> 2 & 1) * 8;
-            Planes<kIn> cut[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) cut[y] = planes_of(x[y]);
-#pragma unroll
-            for (int plane = 0; plane < kIn; ++plane) {
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const u32x4 w = cut[y].p[plane];
-                    *reinterpret_cast<uint2 *>(low + plane * C::kPlane + y * C::kRowBytes) = make_uint2(w[0], w[1]);
-                    *reinterpret_cast<uint2 *>(high + plane * C::kPlane + y * C::kRowBytes) = make_uint2(w[2], w[3]);
-                }
-                if (of == 0)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
-                        *reinterpret_cast<uint2 *>(columns + plane * C::kTransposed + e * 144) =
-                            make_uint2(__builtin_amdgcn_perm(cut[1].p[plane][e / 2], cut[0].p[plane][e / 2], pick), __builtin_amdgcn_perm(cut[3].p[plane][e / 2], cut[2].p[plane][e / 2], pick));
-                    }
             }
         }
+    };
+    auto put_transposed = [&](const V8 (&x)[kPieces][kRows]) {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) {
+            const int c = c0 + m * (kThreads / kAcross), four = kRows * r >> 2;          // (group of four rows)
+            unsigned char *const to = lds + C::kT + 8 * c * 144 + ((four >> 3) * 4 + (four & 3)) * 16 + (four >> 2 & 1) * 8 + (kRows * r & 3) * 2;
+            Planes<kIn> p[kRows];
+#pragma unroll
+            for (int y = 0; y < kRows; ++y) p[y] = cut(x[m][y], c);
+#pragma unroll
+            for (int plane = 0; plane < kIn; ++plane)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    uint32_t w[kRows / 2];
+#pragma unroll
+                    for (int y = 0; y < kRows; y += 2) w[y / 2] = __builtin_amdgcn_perm(p[y + 1].p[plane][e / 2], p[y].p[plane][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+                    unsigned char *const at = to + plane * C::kTransposed + e * 144;
+                    if constexpr (kRows == 4) *reinterpret_cast<uint2 *>(at) = make_uint2(w[0], w[1]);
+                    else *reinterpret_cast<uint32_t *>(at) = w[0];
+                }
+        }
+    };
+    auto put_rest = [&] {
 #pragma unroll
         for (int m = 0; m < kBlocks / 2; ++m) {
             const int at = m * 4 + wave, of = at / kBlocks, block = at % kBlocks, row = row_of(block), c = block - block_of(row, 0);
             unsigned char *to = lds + C::kPairsAt + ((of * kPairs + pair_of(row, c >> 1)) * 3 * 64 + lane) * 16 + (c & 1) * 8;
-            f32x4 x = next.blocks[m];
+            f32x4 x = blocks_next[m];
 #pragma unroll
             for (int plane = 0; plane < 3; ++plane) {
                 *reinterpret_cast<uint2 *>(to + plane * 1024) = make_uint2(upper(x[0], x[1]), upper(x[2], x[3]));
@@ -468,7 +476,11 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
                 for (int e = 0; e < 4; ++e) x[e] = rest(x[e]);
             }
         }
-        if (tid < 2 * kChunk) reinterpret_cast<float *>(lds + C::kDecays)[tid] = next.decay;
+        reinterpret_cast<float *>(lds + C::kDecays)[tid % (2 * kChunk)] = decay_next;
+        typedef T Two __attribute__((ext_vector_type(2)));
+        unsigned char *const to = lds + C::kV + (tid >> 5) * 8 * C::kColumn + (tid & 31) * sizeof(Two);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<Two *>(to + e * C::kColumn) = Two{values_next[0][e], values_next[1][e]};
     };
     auto rows = [&](int of, int m, int k) {              // K or Q, rows 16 m .., channels 32 k ..
         Planes<kIn> p;
@@ -492,7 +504,8 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     };
     const float *decays = reinterpret_cast<const float *>(lds + C::kDecays);
 
-    fetch(0);
+    fetch_rows(0);
+    fetch_rest(0);
     for (int at = tid; at < 2 * kPairs * 3 * 64; at += kThreads) reinterpret_cast<u32x4 *>(lds + C::kPairsAt)[at] = u32x4{0, 0, 0, 0};      // (pairs' blocks above the diagonal)
     float *state = a.state + (b * a.Hv + h) * a.dk * a.dv + (in ? col : 0);
     f32x4 S[NK];
@@ -500,16 +513,28 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     for (int k = 0; k < NK; ++k)
 #pragma unroll
         for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; S[k][v] = row < a.dk ? state[(int64_t)row * a.dv] : 0.f; }
+    __syncthreads();
+    auto keep = [&] {
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m)
+#pragma unroll
+            for (int y = 0; y < kRows; ++y) keys_now[m][y] = keys_next[m][y];
+    };
+    put_rows(keys_next, 0);
+    put_rows(queries_next, 1);
+    put_rest();
+    keep();
+    fetch_rows(min((int64_t)kChunk, end));
+    __syncthreads();
 #pragma unroll 1
     for (int64_t done = 0; done < n; done += kChunk) {
-        const int live = (int)min((int64_t)kChunk, n - done);
-        __syncthreads();                              // nobody reads the chunk before any more
-        put();
-        __syncthreads();
-        if (done + kChunk < n) fetch(done + kChunk);
-        f32x4 kS[4], O[4], U[4];
+        const int64_t next = min(done + kChunk, end);
+        // K S and Q S; K^T of this chunk into LDS
+        fetch_rest(next);
+        put_transposed(keys_now);
+        f32x4 kS[4], O[4], U[4], R[4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) { kS[m] = O[m] = U[m] = f32x4{0, 0, 0, 0}; }
+        for (int m = 0; m < 4; ++m) { kS[m] = O[m] = f32x4{0, 0, 0, 0}; }
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
             const Planes<3> s = planes<3>(S[2 * k], S[2 * k + 1]);
@@ -517,14 +542,19 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
             add_planes(kS, keys, s);
             add_planes<true>(O, queries, s);
         }
-        f32x4 R[4];
+        __syncthreads();
+        // U and O; K and Q of the next chunk into LDS
+        put_rows(keys_next, 0);
+        put_rows(queries_next, 1);
+        keep();
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const auto v = *reinterpret_cast<const typename Some<T, 4>::type *>(lds + C::kV + (wave * 16 + i) * C::kColumn + (16 * m + 4 * g) * sizeof(T));
+            const V4 v = *reinterpret_cast<const V4 *>(lds + C::kV + (wave * 16 + i) * C::kColumn + (16 * m + 4 * g) * sizeof(T));
             const f32x4 eG = *reinterpret_cast<const f32x4 *>(decays + 16 * m + 4 * g);
 #pragma unroll
             for (int c = 0; c < 4; ++c) R[m][c] = (float)v[c] - eG[c] * kS[m][c];
             O[m] *= decays[16 * m + i] * a.scale;
+            U[m] = f32x4{0, 0, 0, 0};
         }
         auto below = [&](auto swapped, f32x4 (&acc)[4], int of, const f32x4 (&x)[4]) {         // acc += T x, or (P x)^T
             const Planes<3> left[4] = {pair(of, 0, 0), pair(of, 1, 0), pair(of, 2, 0), pair(of, 3, 0)};
@@ -536,21 +566,25 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
         };
         below(std::false_type{}, U, 0, R);
         below(std::true_type{}, O, 1, U);
+        const float last = decays[kChunk - 1];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) U[m] *= *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
+        __syncthreads();
+        // S; T, P and V of the next chunk into LDS, K and Q of the one after that on the way (behind the stores, which are waited for with them)
+        put_rest();
         T *const o = (T *)a.o + ((first + done) * a.Hv + h) * a.dv;
-        const int from = col0 + wave * 16 + 4 * g;
+        const int live = (int)min((int64_t)kChunk, n - done), from = col0 + wave * 16 + 4 * g;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             if (16 * m + i >= live) break;
             T *const to = o + ((16 * m + i) * (uint32_t)(a.Hv * a.dv) + from);
-            if (WIDE) { if (from < a.dv) *reinterpret_cast<typename Some<T, 4>::type *>(to) = __builtin_convertvector(O[m], typename Some<T, 4>::type); }
+            if (WIDE) { if (from < a.dv) *reinterpret_cast<V4 *>(to) = __builtin_convertvector(O[m], V4); }
             else {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) if (from + c < a.dv) to[c] = (T)O[m][c];
             }
         }
-        const float last = decays[kChunk - 1];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) U[m] *= *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
+        fetch_rows(min(next + kChunk, end));
         const Planes<3> u[2] = {planes<3>(U[0], U[1]), planes<3>(U[2], U[3])};
 #pragma unroll
         for (int k = 0; k < NK; k += 2) {
@@ -562,6 +596,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
             }
             S[k] = two[0]; S[k + 1] = two[1];
         }
+        __syncthreads();
     }
     if (in)
 #pragma unroll
@@ -676,7 +711,7 @@ int launch(hipStream_t st, const DeltaArgs &a, f32x4 *slots) {
     hipLaunchKernelGGL((delta_within_kernel<T, WIDE>), dim3((unsigned)(a.T / kChunk + a.B), (unsigned)a.Hv), dim3(256), 0, st, a, slots);
     RWKV_CHECK_LAUNCH("delta_within_kernel");
     return by_channels(a.dk, [&](auto nk) {
-        constexpr int NK = decltype(nk)::value;
+        constexpr int NK = decltype(nk)::value < 4 ? 4 : decltype(nk)::value;
         constexpr bool kInPlanes = Chunks<T, NK>::kBytes <= 160 * 1024;
         constexpr size_t bytes = kInPlanes ? Chunks<T, NK>::kBytes : 2 * kChunk * (NK * 16 + 4) * 4;
         constexpr auto kernel = [] { if constexpr (kInPlanes) return &delta_chunks_kernel<T, NK, WIDE>; else return &delta_chunks_f32_kernel<T, NK, WIDE>; }();
