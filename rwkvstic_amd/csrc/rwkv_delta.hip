@@ -21,8 +21,8 @@ namespace rwkv {
 namespace {
 
 struct DeltaArgs {
-    int64_t T, B;
-    int Hk, Hv, dk, dv;
+    int64_t T, B, each;                   // each: rows of a sequence where there are no starts
+    int share, Hv, dk, dv;                // share: value heads to a key head
     const void *q, *k, *v; int64_t q_stride, k_stride, v_stride;
     const float *g, *beta;
     float scale;
@@ -33,7 +33,7 @@ struct DeltaArgs {
 
 // First row and number of rows of sequence b, cut to the rows there are.
 __device__ __forceinline__ void rows_of(const DeltaArgs &a, int64_t b, int64_t &first, int64_t &n) {
-    if (!a.starts) { n = a.T / a.B; first = b * n; return; }
+    if (!a.starts) { n = a.each; first = b * n; return; }
     const int64_t lo = a.starts[b], hi = a.starts[b + 1];
     first = min(max(lo, (int64_t)0), a.T);
     n = max(min(hi, a.T) - first, (int64_t)0);
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(256) delta_steps_kernel(DeltaArgs a, int tiles
     const int64_t job = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (job >= a.B * a.Hv * tiles) return;
     const int lane = threadIdx.x & 63, r = lane & 15, col = (int)(job % tiles) * 16 + (lane >> 4) * 4;
-    const int h = (int)(job / tiles % a.Hv), hk = h / (a.Hv / a.Hk);
+    const int h = (int)(job / tiles % a.Hv), hk = h / a.share;
     const int64_t b = job / tiles / a.Hv;
     int64_t first, n;
     rows_of(a, b, first, n);
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
     __shared__ float s_beta[kChunk];
     __shared__ __align__(16) float s_A[kChunk][kChunk + 4], s_X[4][16][20];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
-    const int h = blockIdx.y, hk = h / (a.Hv / a.Hk);
+    const int h = blockIdx.y, hk = h / a.share;
     // the last sequence whose places begin here or before
     const int64_t place = blockIdx.x;
     int64_t b = -1;
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     constexpr int kIn = C::kIn, kRows = C::kRows, kPieces = C::kPieces, kAcross = kChunk / kRows;
     extern __shared__ __align__(16) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
-    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / (a.Hv / a.Hk);
+    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / a.share;
     const int64_t b = blockIdx.x / groups / a.Hv;
     const int col0 = (int)(blockIdx.x % groups) * 64, col = col0 + wave * 16 + i;
     const bool in = col < a.dv;
@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     V8 keys_next[kPieces][kRows], queries_next[kPieces][kRows], keys_now[kPieces][kRows], values_next[2];
     f32x4 blocks_next[kBlocks / 2];
     float decay_next;
-    const int r = tid % kAcross, c0 = tid / kAcross;
+    // (four neighbouring lanes to a row: the memory pipeline takes four 16-byte loads of one line at a time)
+    const int r = (tid >> 2) % kAcross, c0 = (tid & 3) + tid / (4 * kAcross) * 4, r_values = tid >> 2 & 31, c_values = (tid & 3) + (tid >> 7) * 4;
     auto fetch_rows = [&](int64_t done) {
 #pragma unroll
         for (int m = 0; m < kPieces; ++m) {
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
 #pragma unroll
         for (int m = 0; m < kBlocks / 2; ++m) blocks_next[m] = units[m * kThreads + tid];
         decay_next = reinterpret_cast<const float *>(units + kUnitG)[tid % (2 * kChunk)];
-        piece(values_next, (const T *)a.v + (int64_t)h * a.dv + col0, a.v_stride, done, 2, tid & 31, tid >> 5, a.dv - col0);
+        piece(values_next, (const T *)a.v + (int64_t)h * a.dv + col0, a.v_stride, done, 2, r_values, c_values, a.dv - col0);
     };
     auto cut = [&](const V8 &x, int c) { return planes_of(WIDE && 8 * c >= a.dk ? V8((T)0.f) : x); };
     auto put_rows = [&](const V8 (&x)[kPieces][kRows], int of) {
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
         }
         reinterpret_cast<float *>(lds + C::kDecays)[tid % (2 * kChunk)] = decay_next;
         typedef T Two __attribute__((ext_vector_type(2)));
-        unsigned char *const to = lds + C::kV + (tid >> 5) * 8 * C::kColumn + (tid & 31) * sizeof(Two);
+        unsigned char *const to = lds + C::kV + c_values * 8 * C::kColumn + r_values * sizeof(Two);
 #pragma unroll
         for (int e = 0; e < 8; ++e) *reinterpret_cast<Two *>(to + e * C::kColumn) = Two{values_next[0][e], values_next[1][e]};
     };
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(256) delta_chunks_f32_kernel(DeltaArgs a, cons
     extern __shared__ __align__(16) unsigned char smem[];
     float *ks = reinterpret_cast<float *>(smem), *qs = ks + kChunk * kRow;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / (a.Hv / a.Hk);
+    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / a.share;
     const int64_t b = blockIdx.x / groups / a.Hv;
     const int col = (int)(blockIdx.x % groups) * (int)(blockDim.x >> 2) + wave * 16 + i;
     const bool in = col < a.dv;
@@ -754,7 +755,7 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
         if (!workspace || workspace_bytes < rwkv_delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv))
             return set_error(RWKV_ERR_WORKSPACE, "rwkv_delta_rule: workspace too small");
     }
-    const DeltaArgs a{T, B, (int)Hk, (int)Hv, (int)dk, (int)dv, q, k, v, q_stride, k_stride, v_stride, g, beta, scale, starts, state, o};
+    const DeltaArgs a{T, B, T / B, (int)(Hv / Hk), (int)Hv, (int)dk, (int)dv, q, k, v, q_stride, k_stride, v_stride, g, beta, scale, starts, state, o};
     const size_t size = type_bytes(type);
     auto fits = [&](const void *at, int64_t stride, int64_t channels) { return ((uintptr_t)at | (uintptr_t)(stride * size) | (uintptr_t)(channels * size)) % 16 == 0; };
     // (heads of whole 16 bytes, which are also what a lane of delta_steps_kernel takes at a time, or multiples of it)

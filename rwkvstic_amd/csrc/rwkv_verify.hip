@@ -41,10 +41,33 @@ struct VerifyArgs {
     Verdict *verdict;                // [B]
 };
 
+// e^d for d <= 0 (anything that is not a number or below -800: 0), to 2^-47 or so: the exponent in 32nds of log2 e from a table, the
+// rest by its series (P. T. P. Tang, ACM TOMS 15, 1989).  Half the instructions of exp(), which takes longer than the logits
+// take to come; 2^-47 moves one draw in 10^9.
+struct Exp {
+    const double *table;                             // LDS: 2^(i/32)
+    __device__ __forceinline__ double operator()(double d) const {
+        constexpr double kMagic = 6755399441055744.0;                        // 3 * 2^51: adding it rounds to a whole number
+        const double y = fmax(d, -800.0) * 46.166241308446829;            // 32 log2 e (a d that is no number gives way to -800)
+        const double z = y + kMagic, f = y - (z - kMagic);
+        const int n = (int)__double_as_longlong(z);
+        double p = fma(f, 3.9737099845494161e-11, 9.1725627018246432e-09);          // (ln 2 / 32)^k / k!
+        p = fma(f, p, 1.6938509724371820e-06);
+        p = fma(f, p, 2.3459619820224679e-04);
+        p = fma(f, p, 2.1660849392498291e-02);
+        p = fma(f, p, 1.0);
+        const double e = ldexp(table[n & 31] * p, n >> 5);
+        return d > -800.0 ? e : 0.0;
+    }
+};
+__device__ __forceinline__ Exp exp_table(double (&table)[32]) {              // (before a barrier)
+    if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32);
+    return {table};
+}
+
 // A logit's weight beside the largest; NaN and -infinity have none, and where the largest is +infinity the others have none.
-__device__ __forceinline__ double weight(double x, double max, double inv_temp) {
-    const double d = (x - max) * inv_temp;
-    return d == d ? exp(d) : x == max && x > -INFINITY ? 1.0 : 0.0;
+__device__ __forceinline__ double weight(Exp e, double x, double max, double inv_temp) {
+    return max == INFINITY ? (x == max ? 1.0 : 0.0) : e((x - max) * inv_temp);
 }
 
 __device__ __forceinline__ void better(double &x, int &i, double y, int j) {
@@ -60,8 +83,10 @@ template <typename Real, bool GREEDY>
 __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
     using Vec = typename Wide<Real>::type;
     constexpr int E = 16 / sizeof(Real);
-    __shared__ double s_max[kWaves], red[kWaves];
+    __shared__ double s_max[kWaves], red[kWaves], s_exp[32];
     __shared__ int s_first[kWaves];
+    const Exp e = exp_table(s_exp);
+    __syncthreads();
     const int64_t targets = a.B * (a.K + 1), at = blockIdx.x, of = at < targets ? a.K + 1 : a.K, row = at < targets ? at : at - targets;
     const Real *x = at < targets ? (const Real *)a.logits + row / of * a.seq + row % of * a.row
                                  : (const Real *)a.draft + row / of * a.draft_seq + row % of * a.draft_row;
@@ -93,12 +118,17 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
             for (int k = 0; k < kPer / E; ++k)
 #pragma unroll
                 for (int e = 0; e < E; ++e) top = fmax(top, (double)v[k][e]);
-            s *= weight(m, top, a.inv_temp);
+            s *= weight(e, m, top, a.inv_temp);
             m = top;
+            if (m == INFINITY) {
 #pragma unroll
-            for (int k = 0; k < kPer / E; ++k)
+                for (int k = 0; k < kPer; ++k) s += v[k / E][k % E] == INFINITY ? 1.0 : 0.0;
+            } else {
+                double part[2] = {0.0, 0.0};
 #pragma unroll
-                for (int e = 0; e < E; ++e) s += weight(v[k][e], m, a.inv_temp);
+                for (int k = 0; k < kPer; ++k) part[k & 1] += e(((double)v[k / E][k % E] - m) * a.inv_temp);
+                s += part[0] + part[1];
+            }
         }
     }
     RowStat *to = a.stat + at * a.segments + blockIdx.y;
@@ -116,17 +146,10 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
         if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
         __syncthreads();
         for (int w = 0; w < kWaves; ++w) m = fmax(m, s_max[w]);
-        double sum[1] = {s * weight(own, m, a.inv_temp)};
+        double sum[1] = {s * weight(e, own, m, a.inv_temp)};
         block_sum(sum, red);
         if (threadIdx.x == 0) *to = {m, sum[0], 0, 0};
     }
-}
-
-// A row's segments put together.
-__device__ __forceinline__ void whole_row(const VerifyArgs &a, const RowStat *s, double &max, double &sum) {
-    max = -INFINITY; sum = 0.0;
-    for (int i = 0; i < a.segments; ++i) max = fmax(max, s[i].max);
-    for (int i = 0; i < a.segments; ++i) sum += s[i].sum * weight(s[i].max, max, a.inv_temp);
 }
 
 __device__ __forceinline__ int drafts_of(const VerifyArgs &a, int64_t b) { return a.lengths ? max(0, min((int)a.K, a.lengths[b])) : (int)a.K; }
@@ -137,66 +160,85 @@ struct Left {
     const Real *x, *y;
     int64_t gone;                    // drafts without a distribution: the one that was refused
     Verdict v;
-    double inv_temp;
-    __device__ Left(const VerifyArgs &a, int64_t b, const Verdict &v_) : v(v_), inv_temp(a.inv_temp) {
+    double inv_temp, per_p, per_q;
+    Exp e;
+    __device__ Left(const VerifyArgs &a, int64_t b, const Verdict &v_, Exp e_) : v(v_), inv_temp(a.inv_temp), e(e_) {
         x = (const Real *)a.logits + b * a.seq + v.n * a.row;
         y = a.draft && v.left ? (const Real *)a.draft + b * a.draft_seq + v.n * a.draft_row : nullptr;
         gone = v.left ? a.drafts[b * a.K + v.n] : -1;
+        per_p = 1.0 / v.p_sum;
+        per_q = v.q_sum > 0 ? 1.0 / v.q_sum : 0.0;
     }
-    __device__ __forceinline__ double at(int64_t j) const {
-        const double p = weight(x[j], v.p_max, inv_temp) / v.p_sum;
+    // (px, qx: the logits at j)
+    __device__ __forceinline__ double of(double px, double qx, int64_t j) const {
+        const double p = weight(e, px, v.p_max, inv_temp) * per_p;
         if (!v.left) return p;
-        const double q = !y ? (j == gone ? 1.0 : 0.0) : v.q_sum > 0 ? weight(y[j], v.q_max, inv_temp) / v.q_sum : 0.0;
-        return fmax(p - q, 0.0);
+        return fmax(p - (y ? weight(e, qx, v.q_max, inv_temp) * per_q : j == gone ? 1.0 : 0.0), 0.0);
     }
 };
 
-// A workgroup per sequence and segment; each finds out for itself how many drafts are accepted, a thread to a draft.
+// A workgroup per sequence and segment; each finds out for itself how many drafts are accepted: rows' segments put together by
+// 16 lanes (64 where there are more), then a thread to a draft.
 template <typename Real>
 __global__ void __launch_bounds__(kVT) verify_left_kernel(VerifyArgs a) {
-    __shared__ double red[kWaves];
+    __shared__ double red[kWaves], s_exp[32], s_max[2 * kMaxDrafts + 1], s_sum[2 * kMaxDrafts + 1];
     __shared__ Verdict s_v;
     const int64_t b = blockIdx.x;
-    const int tid = threadIdx.x, count = drafts_of(a, b);
-    const RowStat *ps = a.stat + b * (a.K + 1) * a.segments, *qs = a.stat + (a.B * (a.K + 1) + b * a.K) * a.segments;
+    const int tid = threadIdx.x, count = drafts_of(a, b), K = (int)a.K;
+    const Exp e = exp_table(s_exp);
+    const RowStat *ps = a.stat + b * (K + 1) * a.segments, *qs = a.stat + (a.B * (K + 1) + b * K) * a.segments;
+    // the drafts' own logits, on the way meanwhile
+    int64_t d = -1;
+    double px = -INFINITY, qx = -INFINITY, u = 0.0;
+    if (tid < count) {
+        d = a.drafts[b * K + tid];
+        u = a.u[b * (K + 1) + tid];
+        if (d >= 0 && d < a.V) {
+            px = ((const Real *)a.logits)[b * a.seq + tid * a.row + d];
+            if (a.draft) qx = ((const Real *)a.draft)[b * a.draft_seq + tid * a.draft_row + d];
+        } else d = -1;
+    }
+    __syncthreads();
+    const int lanes = a.segments <= 16 ? 16 : 64, rows = K + 1 + (a.draft ? K : 0);
+    for (int row = tid / lanes; row < (int)round_up(rows, kVT / lanes); row += kVT / lanes) {
+        const int i = tid % lanes;
+        const bool in = row < rows && i < a.segments;
+        const RowStat *s = (row <= K ? ps + row * a.segments : qs + (row - K - 1) * a.segments) + i;
+        const double own = in ? s->max : -INFINITY;
+        double max = own, sum = in ? s->sum : 0.0;
+        for (int off = lanes / 2; off >= 1; off >>= 1) max = fmax(max, __shfl_xor(max, off, 64));
+        sum *= weight(e, own, max, a.inv_temp);
+        for (int off = lanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        if (in && i == 0) { s_max[row] = max; s_sum[row] = sum; }
+    }
+    __syncthreads();
     if (tid < 64) {
-        bool taken = true;                            // (beyond the drafts nothing refuses)
-        if (tid < count) {
-            const int64_t d = a.drafts[b * a.K + tid];
-            taken = false;
-            if (d >= 0 && d < a.V) {
-                double max, sum, q = 1.0;
-                whole_row(a, ps + tid * a.segments, max, sum);
-                const double p = sum > 0 ? weight(((const Real *)a.logits)[b * a.seq + tid * a.row + d], max, a.inv_temp) / sum : 0.0;
-                if (a.draft) {
-                    whole_row(a, qs + tid * a.segments, max, sum);
-                    q = sum > 0 ? weight(((const Real *)a.draft)[b * a.draft_seq + tid * a.draft_row + d], max, a.inv_temp) / sum : 0.0;
-                }
-                taken = (double)a.u[b * (a.K + 1) + tid] * q < p;
-            }
+        bool taken = tid >= count;                    // (beyond the drafts nothing refuses)
+        if (d >= 0 && s_sum[tid] > 0) {
+            const double p = weight(e, px, s_max[tid], a.inv_temp) / s_sum[tid];
+            const double q = !a.draft ? 1.0 : s_sum[K + 1 + tid] > 0 ? weight(e, qx, s_max[K + 1 + tid], a.inv_temp) / s_sum[K + 1 + tid] : 0.0;
+            taken = u * q < p;
         }
         const unsigned long long refused = __ballot(!taken);
-        const int n = refused ? min(__ffsll(refused) - 1, count) : count;
         if (tid == 0) {
-            Verdict v{0, 0, -INFINITY, 0, n, n < count};
-            whole_row(a, ps + n * a.segments, v.p_max, v.p_sum);
-            if (v.left && a.draft) whole_row(a, qs + n * a.segments, v.q_max, v.q_sum);
-            s_v = v;
-            if (blockIdx.y == 0) a.verdict[b] = v;
+            const int n = refused ? min(__ffsll(refused) - 1, count) : count;
+            const bool left = n < count, of_drafts = left && a.draft;
+            s_v = {s_max[n], s_sum[n], of_drafts ? s_max[K + 1 + n] : -INFINITY, of_drafts ? s_sum[K + 1 + n] : 0.0, n, left};
+            if (blockIdx.y == 0) a.verdict[b] = s_v;
         }
     }
     __syncthreads();
     const Verdict v = s_v;
     if (!v.left || !(v.p_sum > 0)) return;
-    const Left<Real> left(a, b, v);
+    const Left<Real> left(a, b, v, e);
     const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
     double s[1] = {0.0};
     for (int64_t j = j0; j < j1; j += kChunk) {
-#pragma unroll 4
-        for (int k = 0; k < kPer; ++k) {
-            const int64_t i = j + k * kVT + tid;
-            if (i < j1) s[0] += left.at(i);
-        }
+        Real x[kPer], y[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) { const int64_t i = min(j + k * kVT + tid, j1 - 1); x[k] = left.x[i]; y[k] = left.y ? left.y[i] : (Real)0; }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) { const int64_t i = j + k * kVT + tid; s[0] += i < j1 ? left.of(x[k], y[k], i) : 0.0; }
     }
     block_sum(s, red);
     if (tid == 0) a.sums[b * a.segments + blockIdx.y] = s[0];
@@ -208,49 +250,51 @@ __device__ __forceinline__ void answer(const VerifyArgs &a, int64_t b, int n, in
     if (threadIdx.x == 0) a.accepted[b] = n;
 }
 
+__device__ __forceinline__ double upto(double v, int lane) {                 // the lanes' values up to this one's
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) { const double o = __shfl_up(v, off, 64); if (lane >= off) v += o; }
+    return v;
+}
+
 // A workgroup per sequence.
 template <typename Real>
 __global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
-    __shared__ double s_sums[kSegments], s_wave[kWaves], s_aim, s_before;
+    __shared__ double s_wave[kWaves], s_aim, s_before, s_exp[32];
     __shared__ int s_segment, s_left, s_hit, s_last;
     const int64_t b = blockIdx.x;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const Exp e = exp_table(s_exp);
     Verdict v = a.verdict[b];
+    __syncthreads();
     if (!(v.p_sum > 0)) { answer(a, b, v.n, -1); return; }
-    for (int round = v.left ? 0 : 1; round < 2; ++round) {              // what is left; p itself, where that is nothing
+    if (tid < 64) {
+        // the segment that passes the aim first, or the last that has anything: of what is left, or of p itself where that is nothing
         const RowStat *ps = a.stat + (b * (a.K + 1) + v.n) * a.segments;
-        __syncthreads();
-        if (tid < a.segments) s_sums[tid] = round == 0 ? a.sums[b * a.segments + tid] : ps[tid].sum * weight(ps[tid].max, v.p_max, a.inv_temp) / v.p_sum;
-        __syncthreads();
-        if (tid == 0) {
-            double all = 0.0, run = 0.0;
-            for (int i = 0; i < a.segments; ++i) all += s_sums[i];
-            const double aim = (double)a.u[b * (a.K + 1) + a.K] * all;
-            int at = -1;
-            for (int i = 0; i < a.segments; ++i) {                      // the first segment that passes the aim, or the last that has anything
-                if (s_sums[i] > 0.0) { at = i; s_before = run; }
-                run += s_sums[i];
-                if (run > aim && s_sums[i] > 0.0) break;
-            }
-            s_aim = aim; s_segment = at; s_left = round == 0; s_hit = 0x7fffffff; s_last = -1;
-        }
-        __syncthreads();
-        if (s_segment >= 0) break;
+        const double of_p = lane < a.segments ? ps[lane].sum * weight(e, ps[lane].max, v.p_max, a.inv_temp) / v.p_sum : 0.0;
+        double own = v.left && lane < a.segments ? a.sums[b * a.segments + lane] : 0.0;
+        bool left = v.left && __ballot(own > 0.0);
+        if (!left) own = of_p;
+        const double run = upto(own, lane), aim = (double)a.u[b * (a.K + 1) + a.K] * __shfl(run, 63, 64);
+        const unsigned long long any = __ballot(own > 0.0), over = __ballot(own > 0.0 && run > aim);
+        const int at = over ? __ffsll(over) - 1 : 63 - __clzll(any);          // (p has something: its sum is over 0)
+        if (lane == at) { s_segment = at; s_before = run - own; s_aim = aim; s_left = left; s_hit = 0x7fffffff; s_last = -1; }
     }
+    __syncthreads();
     v.left = s_left;
-    const Left<Real> left(a, b, v);
+    const Left<Real> left(a, b, v, e);
     const int64_t j0 = s_segment * a.segment, j1 = min(a.V, j0 + a.segment);
     const double aim = s_aim;
     double before = s_before;
     for (int64_t j = j0; j < j1; j += kChunk) {                         // (one chunk, unless the vocabulary is over kSegments of them)
         const int64_t i0 = j + tid * kPer;
         double w[kPer], own = 0.0;
+        Real x[kPer], y[kPer];
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) { w[k] = i0 + k < j1 ? left.at(i0 + k) : 0.0; own += w[k]; }
-        double run = own;
+        for (int k = 0; k < kPer; ++k) { const int64_t i = min(i0 + k, j1 - 1); x[k] = left.x[i]; y[k] = left.y ? left.y[i] : (Real)0; }
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) { const double o = __shfl_up(run, off, 64); if ((tid & 63) >= off) run += o; }
-        if ((tid & 63) == 63) s_wave[tid >> 6] = run;
+        for (int k = 0; k < kPer; ++k) { w[k] = i0 + k < j1 ? left.of(x[k], y[k], i0 + k) : 0.0; own += w[k]; }
+        double run = upto(own, lane);
+        if (lane == 63) s_wave[tid >> 6] = run;
         __syncthreads();
         double after = before;
         run += before - own;
