@@ -78,11 +78,32 @@ template <typename Real> struct Wide;                // 16 bytes of logits, wher
 template <> struct Wide<double> { typedef double type __attribute__((ext_vector_type(2), aligned(8))); };
 template <> struct Wide<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
 
+// A chunk of a row, 16 bytes a load: thread t has tokens j + (256 k + t) E + e as its element k E + e; -infinity behind the end.
+template <typename Real>
+__device__ __forceinline__ void load_chunk(Real (&to)[kPer], const Real *x, int64_t j, int64_t end) {
+    using Vec = typename Wide<Real>::type;
+    constexpr int E = 16 / sizeof(Real);
+#pragma unroll
+    for (int k = 0; k < kPer / E; ++k) {
+        const int64_t i = j + (k * kVT + (int)threadIdx.x) * E;
+        Vec v;
+        if (i + E <= end) v = *reinterpret_cast<const Vec *>(x + i);
+        else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = i + e < end ? x[i + e] : (Real)-INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) to[k * E + e] = v[e];
+    }
+}
+template <typename Real> __device__ __forceinline__ int in_chunk(int k) {              // which of the chunk's tokens element k is
+    constexpr int E = 16 / sizeof(Real);
+    return (k / E * kVT + (int)threadIdx.x) * E + k % E;
+}
+
 // A workgroup per row and segment.
 template <typename Real, bool GREEDY>
 __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
-    using Vec = typename Wide<Real>::type;
-    constexpr int E = 16 / sizeof(Real);
     __shared__ double s_max[kWaves], red[kWaves], s_exp[32];
     __shared__ int s_first[kWaves];
     const Exp e = exp_table(s_exp);
@@ -94,39 +115,24 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
     double m = -INFINITY, s = 0.0;
     int first = -1;
     for (int64_t j = j0; j < j1; j += kChunk) {
-        Vec v[kPer / E];
-#pragma unroll
-        for (int k = 0; k < kPer / E; ++k) {
-            const int64_t i = j + (k * kVT + (int)threadIdx.x) * E;
-            if (i + E <= j1) v[k] = *reinterpret_cast<const Vec *>(x + i);
-            else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[k][e] = i + e < j1 ? x[i + e] : (Real)-INFINITY;
-            }
-        }
+        Real v[kPer];
+        load_chunk(v, x, j, j1);
         if (GREEDY) {
 #pragma unroll
-            for (int k = 0; k < kPer / E; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int i = (int)j + (k * kVT + (int)threadIdx.x) * E + e;
-                    if ((double)v[k][e] > m) { m = v[k][e]; first = i; }
-                }
+            for (int k = 0; k < kPer; ++k) if ((double)v[k] > m) { m = v[k]; first = (int)j + in_chunk<Real>(k); }
         } else {
             double top = m;
 #pragma unroll
-            for (int k = 0; k < kPer / E; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) top = fmax(top, (double)v[k][e]);
+            for (int k = 0; k < kPer; ++k) top = fmax(top, (double)v[k]);
             s *= weight(e, m, top, a.inv_temp);
             m = top;
             if (m == INFINITY) {
 #pragma unroll
-                for (int k = 0; k < kPer; ++k) s += v[k / E][k % E] == INFINITY ? 1.0 : 0.0;
+                for (int k = 0; k < kPer; ++k) s += v[k] == INFINITY ? 1.0 : 0.0;
             } else {
                 double part[2] = {0.0, 0.0};
 #pragma unroll
-                for (int k = 0; k < kPer; ++k) part[k & 1] += e(((double)v[k / E][k % E] - m) * a.inv_temp);
+                for (int k = 0; k < kPer; ++k) part[k & 1] += e(((double)v[k] - m) * a.inv_temp);
                 s += part[0] + part[1];
             }
         }
@@ -235,10 +241,10 @@ __global__ void __launch_bounds__(kVT) verify_left_kernel(VerifyArgs a) {
     double s[1] = {0.0};
     for (int64_t j = j0; j < j1; j += kChunk) {
         Real x[kPer], y[kPer];
+        load_chunk(x, left.x, j, j1);
+        if (left.y) load_chunk(y, left.y, j, j1);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) { const int64_t i = min(j + k * kVT + tid, j1 - 1); x[k] = left.x[i]; y[k] = left.y ? left.y[i] : (Real)0; }
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) { const int64_t i = j + k * kVT + tid; s[0] += i < j1 ? left.of(x[k], y[k], i) : 0.0; }
+        for (int k = 0; k < kPer; ++k) s[0] += left.of(x[k], y[k], j + in_chunk<Real>(k));
     }
     block_sum(s, red);
     if (tid == 0) a.sums[b * a.segments + blockIdx.y] = s[0];
@@ -259,7 +265,7 @@ __device__ __forceinline__ double upto(double v, int lane) {                 // 
 // A workgroup per sequence.
 template <typename Real>
 __global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
-    __shared__ double s_wave[kWaves], s_aim, s_before, s_exp[32];
+    __shared__ double s_wave[kWaves], s_aim, s_before, s_exp[32], s_w[kVT][kPer + 1];
     __shared__ int s_segment, s_left, s_hit, s_last;
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -289,10 +295,13 @@ __global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
         const int64_t i0 = j + tid * kPer;
         double w[kPer], own = 0.0;
         Real x[kPer], y[kPer];
+        load_chunk(x, left.x, j, j1);
+        if (left.y) load_chunk(y, left.y, j, j1);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) { const int64_t i = min(i0 + k, j1 - 1); x[k] = left.x[i]; y[k] = left.y ? left.y[i] : (Real)0; }
+        for (int k = 0; k < kPer; ++k) { const int at = in_chunk<Real>(k); s_w[at / kPer][at % kPer] = left.of(x[k], y[k], j + at); }
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) { w[k] = i0 + k < j1 ? left.of(x[k], y[k], i0 + k) : 0.0; own += w[k]; }
+        for (int k = 0; k < kPer; ++k) { w[k] = s_w[tid][k]; own += w[k]; }
         double run = upto(own, lane);
         if (lane == 63) s_wave[tid >> 6] = run;
         __syncthreads();
@@ -315,22 +324,29 @@ __global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
     answer(a, b, v.n, s_hit != 0x7fffffff ? s_hit : s_last);            // (rounding can leave none over the aim: the segment's last that has weight)
 }
 
-// A wavefront per sequence, a lane to a row.
-__global__ void __launch_bounds__(kMaxDrafts + 64) verify_greedy_kernel(VerifyArgs a) {
+// A workgroup per sequence, 16 lanes to a row.
+__global__ void __launch_bounds__(kVT) verify_greedy_kernel(VerifyArgs a) {
     __shared__ int best[kMaxDrafts + 1];
     const int64_t b = blockIdx.x;
-    const int tid = threadIdx.x, count = drafts_of(a, b);
-    if (tid <= a.K) {
-        const RowStat *s = a.stat + (b * (a.K + 1) + tid) * a.segments;
+    const int tid = threadIdx.x, count = drafts_of(a, b), K = (int)a.K;
+    const int64_t d = tid < count ? a.drafts[b * K + tid] : -1;
+    for (int row = tid / 16; row < (int)round_up(K + 1, kVT / 16); row += kVT / 16) {
+        const RowStat *s = a.stat + (b * (K + 1) + min(row, K)) * a.segments;
         double m = -INFINITY;
         int first = -1;
-        for (int i = 0; i < a.segments; ++i) better(m, first, s[i].max, s[i].first);
-        best[tid] = first;
+        for (int i = tid % 16; i < a.segments; i += 16) better(m, first, s[i].max, s[i].first);
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) better(m, first, __shfl_xor(m, off, 64), __shfl_xor(first, off, 64));
+        if (tid % 16 == 0 && row <= K) best[row] = first;
     }
     __syncthreads();
-    int n = 0;
-    while (n < count && best[n] >= 0 && best[n] == a.drafts[b * a.K + n]) ++n;
-    answer(a, b, n, best[n]);
+    __shared__ int s_n;
+    if (tid < 64) {
+        const unsigned long long refused = __ballot(tid < count && !(best[min(tid, K)] >= 0 && best[min(tid, K)] == d));
+        if (tid == 0) s_n = refused ? min(__ffsll(refused) - 1, count) : count;
+    }
+    __syncthreads();
+    answer(a, b, s_n, best[s_n]);
 }
 
 struct VerifyPlan {
@@ -384,7 +400,7 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
         using Real = typename decltype(re)::type;
         if (greedy) {
             hipLaunchKernelGGL((verify_rows_kernel<Real, true>), rows, dim3(kVT), 0, st, a);
-            hipLaunchKernelGGL(verify_greedy_kernel, dim3((unsigned)B), dim3(kMaxDrafts + 64), 0, st, a);
+            hipLaunchKernelGGL(verify_greedy_kernel, dim3((unsigned)B), dim3(kVT), 0, st, a);
         } else {
             hipLaunchKernelGGL((verify_rows_kernel<Real, false>), rows, dim3(kVT), 0, st, a);
             hipLaunchKernelGGL(verify_left_kernel<Real>, left, dim3(kVT), 0, st, a);
