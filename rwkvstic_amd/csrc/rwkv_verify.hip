@@ -12,9 +12,11 @@ namespace rwkv {
 
 namespace {
 
-constexpr int kVT = kThreads;        // threads of a workgroup
-constexpr int kPer = 16;             // tokens a thread takes at a time
-constexpr int kChunk = kVT * kPer;
+constexpr int kVT = kThreads;        // threads of verify_rows_kernel
+constexpr int kPer = 16;             // tokens of a thread
+constexpr int kChunk = kVT * kPer;   // tokens of a workgroup at a time
+// The kernels that draw are short and run once a sequence: what they wait for is their own code, so a thread has four tokens.
+constexpr int kDT = 1024, kFew = kChunk / kDT, kDWaves = kDT / 64;
 constexpr int kSegments = 64;
 constexpr int kMaxDrafts = 64;
 
@@ -37,7 +39,7 @@ struct VerifyArgs {
     int segments;
     int64_t segment;                 // tokens of one, a multiple of kChunk
     RowStat *stat;                   // [B][K+1][segments], then [B][K][segments] of the drafts' logits
-    double *sums;                    // [B][segments]
+    double *sums;                    // [B][segments] of what is left, then [B][segments] of p
     Verdict *verdict;                // [B]
 };
 
@@ -60,8 +62,17 @@ struct Exp {
         return d > -800.0 ? e : 0.0;
     }
 };
+__constant__ const double kTable[32] = {               // 2^(i/32)
+    1.0000000000000000000, 1.0218971486541166782, 1.0442737824274138403, 1.0671404006768236182,
+    1.0905077326652576592, 1.1143867425958925363, 1.1387886347566916537, 1.1637248587775775138,
+    1.1892071150027210667, 1.2152473599804688781, 1.2418578120734840486, 1.2690509571917332226,
+    1.2968395546510096659, 1.3252366431597412946, 1.3542555469368927283, 1.3839098819638319549,
+    1.4142135623730950488, 1.4451808069770466200, 1.4768261459394993114, 1.5091644275934227398,
+    1.5422108254079408236, 1.5759808451078864865, 1.6104903319492543082, 1.6457554781539648445,
+    1.6817928305074290861, 1.7186192981224779156, 1.7562521603732994831, 1.7947090750031071864,
+    1.8340080864093424635, 1.8741676341102999013, 1.9152065613971472939, 1.9571441241754002690};
 __device__ __forceinline__ Exp exp_table(double (&table)[32]) {              // (before a barrier)
-    if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32);
+    if (threadIdx.x < 32) table[threadIdx.x] = kTable[threadIdx.x];
     return {table};
 }
 
@@ -100,6 +111,23 @@ template <typename Real> __device__ __forceinline__ int in_chunk(int k) {       
     constexpr int E = 16 / sizeof(Real);
     return (k / E * kVT + (int)threadIdx.x) * E + k % E;
 }
+// The four tokens i .. i + 3.
+template <typename Real>
+__device__ __forceinline__ void load_few(Real (&to)[kFew], const Real *x, int64_t i, int64_t end) {
+    using Vec = typename Wide<Real>::type;
+    constexpr int E = 16 / sizeof(Real);
+    if (i + kFew <= end) {
+#pragma unroll
+        for (int k = 0; k < kFew; k += E) {
+            const Vec v = *reinterpret_cast<const Vec *>(x + i + k);
+#pragma unroll
+            for (int e = 0; e < E; ++e) to[k + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kFew; ++k) to[k] = i + k < end ? x[i + k] : (Real)-INFINITY;
+    }
+}
 
 // A workgroup per row and segment.
 template <typename Real, bool GREEDY>
@@ -107,16 +135,20 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
     __shared__ double s_max[kWaves], red[kWaves], s_exp[32];
     __shared__ int s_first[kWaves];
     const Exp e = exp_table(s_exp);
-    __syncthreads();
     const int64_t targets = a.B * (a.K + 1), at = blockIdx.x, of = at < targets ? a.K + 1 : a.K, row = at < targets ? at : at - targets;
     const Real *x = at < targets ? (const Real *)a.logits + row / of * a.seq + row % of * a.row
                                  : (const Real *)a.draft + row / of * a.draft_seq + row % of * a.draft_row;
     const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
     double m = -INFINITY, s = 0.0;
     int first = -1;
+    Real next[kPer];
+    load_chunk(next, x, j0, j1);
+    __syncthreads();
     for (int64_t j = j0; j < j1; j += kChunk) {
         Real v[kPer];
-        load_chunk(v, x, j, j1);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[k] = next[k];
+        if (j + kChunk < j1) load_chunk(next, x, j + kChunk, j1);
         if (GREEDY) {
 #pragma unroll
             for (int k = 0; k < kPer; ++k) if ((double)v[k] > m) { m = v[k]; first = (int)j + in_chunk<Real>(k); }
@@ -186,8 +218,8 @@ struct Left {
 // A workgroup per sequence and segment; each finds out for itself how many drafts are accepted: rows' segments put together by
 // 16 lanes (64 where there are more), then a thread to a draft.
 template <typename Real>
-__global__ void __launch_bounds__(kVT) verify_left_kernel(VerifyArgs a) {
-    __shared__ double red[kWaves], s_exp[32], s_max[2 * kMaxDrafts + 1], s_sum[2 * kMaxDrafts + 1];
+__global__ void __launch_bounds__(kDT) verify_left_kernel(VerifyArgs a) {
+    __shared__ double red[kDWaves], s_exp[32], s_max[2 * kMaxDrafts + 1], s_sum[2 * kMaxDrafts + 1];
     __shared__ Verdict s_v;
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, count = drafts_of(a, b), K = (int)a.K;
@@ -206,7 +238,7 @@ __global__ void __launch_bounds__(kVT) verify_left_kernel(VerifyArgs a) {
     }
     __syncthreads();
     const int lanes = a.segments <= 16 ? 16 : 64, rows = K + 1 + (a.draft ? K : 0);
-    for (int row = tid / lanes; row < (int)round_up(rows, kVT / lanes); row += kVT / lanes) {
+    for (int row = tid / lanes; row < (int)round_up(rows, kDT / lanes); row += kDT / lanes) {
         const int i = tid % lanes;
         const bool in = row < rows && i < a.segments;
         const RowStat *s = (row <= K ? ps + row * a.segments : qs + (row - K - 1) * a.segments) + i;
@@ -235,19 +267,31 @@ __global__ void __launch_bounds__(kVT) verify_left_kernel(VerifyArgs a) {
     }
     __syncthreads();
     const Verdict v = s_v;
-    if (!v.left || !(v.p_sum > 0)) return;
+    if (!(v.p_sum > 0)) return;
+    if (tid == 0) {                                   // of p itself, for verify_pick_kernel
+        const RowStat own = ps[v.n * a.segments + blockIdx.y];
+        a.sums[(a.B + b) * a.segments + blockIdx.y] = own.sum * weight(e, own.max, v.p_max, a.inv_temp) / v.p_sum;
+        if (!v.left) a.sums[b * a.segments + blockIdx.y] = 0.0;
+    }
+    if (!v.left) return;
     const Left<Real> left(a, b, v, e);
     const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
-    double s[1] = {0.0};
-    for (int64_t j = j0; j < j1; j += kChunk) {
-        Real x[kPer], y[kPer];
-        load_chunk(x, left.x, j, j1);
-        if (left.y) load_chunk(y, left.y, j, j1);
+    double s = 0.0;
+    for (int64_t j = j0 + tid * kFew; j < j1; j += kChunk) {
+        Real x[kFew], y[kFew];
+        load_few(x, left.x, j, j1);
+        if (left.y) load_few(y, left.y, j, j1);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) s[0] += left.of(x[k], y[k], j + in_chunk<Real>(k));
+        for (int k = 0; k < kFew; ++k) s += left.of(x[k], y[k], j + k);
     }
-    block_sum(s, red);
-    if (tid == 0) a.sums[b * a.segments + blockIdx.y] = s[0];
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < kDWaves; ++w) s += red[w];
+        a.sums[b * a.segments + blockIdx.y] = s;
+    }
 }
 
 // Accepted drafts, the token drawn, -1.
@@ -264,26 +308,25 @@ __device__ __forceinline__ double upto(double v, int lane) {                 // 
 
 // A workgroup per sequence.
 template <typename Real>
-__global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
-    __shared__ double s_wave[kWaves], s_aim, s_before, s_exp[32], s_w[kVT][kPer + 1];
-    __shared__ int s_segment, s_left, s_hit, s_last;
+__global__ void __launch_bounds__(kDT) verify_pick_kernel(VerifyArgs a) {
+    __shared__ double s_wave[kDWaves], s_aim, s_before, s_exp[32];
+    __shared__ int s_segment, s_left, s_hit[kDWaves], s_last[kDWaves];
     const int64_t b = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Exp e = exp_table(s_exp);
     Verdict v = a.verdict[b];
-    __syncthreads();
+    double own = 0.0, of_p = 0.0;
+    if (tid < a.segments) { own = a.sums[b * a.segments + tid]; of_p = a.sums[(a.B + b) * a.segments + tid]; }
+    const double u = a.u[b * (a.K + 1) + a.K];
     if (!(v.p_sum > 0)) { answer(a, b, v.n, -1); return; }
     if (tid < 64) {
         // the segment that passes the aim first, or the last that has anything: of what is left, or of p itself where that is nothing
-        const RowStat *ps = a.stat + (b * (a.K + 1) + v.n) * a.segments;
-        const double of_p = lane < a.segments ? ps[lane].sum * weight(e, ps[lane].max, v.p_max, a.inv_temp) / v.p_sum : 0.0;
-        double own = v.left && lane < a.segments ? a.sums[b * a.segments + lane] : 0.0;
-        bool left = v.left && __ballot(own > 0.0);
+        const bool left = __ballot(own > 0.0);
         if (!left) own = of_p;
-        const double run = upto(own, lane), aim = (double)a.u[b * (a.K + 1) + a.K] * __shfl(run, 63, 64);
+        const double run = upto(own, lane), aim = u * __shfl(run, 63, 64);
         const unsigned long long any = __ballot(own > 0.0), over = __ballot(own > 0.0 && run > aim);
         const int at = over ? __ffsll(over) - 1 : 63 - __clzll(any);          // (p has something: its sum is over 0)
-        if (lane == at) { s_segment = at; s_before = run - own; s_aim = aim; s_left = left; s_hit = 0x7fffffff; s_last = -1; }
+        if (lane == at) { s_segment = at; s_before = run - own; s_aim = aim; s_left = left; }
     }
     __syncthreads();
     v.left = s_left;
@@ -291,37 +334,41 @@ __global__ void __launch_bounds__(kVT) verify_pick_kernel(VerifyArgs a) {
     const int64_t j0 = s_segment * a.segment, j1 = min(a.V, j0 + a.segment);
     const double aim = s_aim;
     double before = s_before;
+    int pick = -1, nearly = -1;                       // rounding can leave no token over the aim: then the segment's last that has weight
     for (int64_t j = j0; j < j1; j += kChunk) {                         // (one chunk, unless the vocabulary is over kSegments of them)
-        const int64_t i0 = j + tid * kPer;
-        double w[kPer], own = 0.0;
-        Real x[kPer], y[kPer];
-        load_chunk(x, left.x, j, j1);
-        if (left.y) load_chunk(y, left.y, j, j1);
+        const int64_t i0 = j + tid * kFew;
+        double w[kFew], own = 0.0;
+        Real x[kFew], y[kFew];
+        load_few(x, left.x, i0, j1);
+        if (left.y) load_few(y, left.y, i0, j1);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) { const int at = in_chunk<Real>(k); s_w[at / kPer][at % kPer] = left.of(x[k], y[k], j + at); }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) { w[k] = s_w[tid][k]; own += w[k]; }
+        for (int k = 0; k < kFew; ++k) { w[k] = left.of(x[k], y[k], i0 + k); own += w[k]; }
         double run = upto(own, lane);
-        if (lane == 63) s_wave[tid >> 6] = run;
+        if (lane == 63) s_wave[wave] = run;
         __syncthreads();
         double after = before;
         run += before - own;
 #pragma unroll
-        for (int q = 0; q < kWaves; ++q) { run += q < (tid >> 6) ? s_wave[q] : 0.0; after += s_wave[q]; }
+        for (int q = 0; q < kDWaves; ++q) { run += q < wave ? s_wave[q] : 0.0; after += s_wave[q]; }
         int hit = 0x7fffffff, last = -1;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
+        for (int k = 0; k < kFew; ++k) {
             run += w[k];
             if (w[k] > 0.0) { last = (int)(i0 + k); if (run > aim && hit == 0x7fffffff) hit = last; }
         }
-        if (hit != 0x7fffffff) atomicMin(&s_hit, hit);
-        if (last >= 0) atomicMax(&s_last, last);
+        // (the first of the wavefront's hits and the last of its tokens with weight; an LDS atomic of 1024 lanes takes 3 us)
+        const unsigned long long hits = __ballot(hit != 0x7fffffff), some = __ballot(last >= 0);
+        if (hits ? lane == __ffsll(hits) - 1 : lane == 0) s_hit[wave] = hit;
+        if (some ? lane == 63 - __clzll(some) : lane == 0) s_last[wave] = last;
         __syncthreads();
-        if (s_hit != 0x7fffffff) break;
+#pragma unroll
+        for (int q = kDWaves - 1; q >= 0; --q) if (s_hit[q] != 0x7fffffff) pick = s_hit[q];
+        if (pick >= 0) break;
+#pragma unroll
+        for (int q = 0; q < kDWaves; ++q) if (s_last[q] >= 0) nearly = s_last[q];
         before = after;
     }
-    answer(a, b, v.n, s_hit != 0x7fffffff ? s_hit : s_last);            // (rounding can leave none over the aim: the segment's last that has weight)
+    answer(a, b, v.n, pick >= 0 ? pick : nearly);
 }
 
 // A workgroup per sequence, 16 lanes to a row.
@@ -357,7 +404,7 @@ struct VerifyPlan {
         segment = round_up(ceil_div(V, kSegments), kChunk);
         segments = (int)ceil_div(V, segment);
         stat_bytes = (size_t)(B * (2 * K + 1) * segments) * sizeof(RowStat);
-        sum_bytes = (size_t)(B * segments) * 8;
+        sum_bytes = (size_t)(2 * B * segments) * 8;
         verdict_bytes = (size_t)B * sizeof(Verdict);
     }
     size_t bytes() const { return stat_bytes + sum_bytes + verdict_bytes; }
@@ -403,8 +450,8 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
             hipLaunchKernelGGL(verify_greedy_kernel, dim3((unsigned)B), dim3(kVT), 0, st, a);
         } else {
             hipLaunchKernelGGL((verify_rows_kernel<Real, false>), rows, dim3(kVT), 0, st, a);
-            hipLaunchKernelGGL(verify_left_kernel<Real>, left, dim3(kVT), 0, st, a);
-            hipLaunchKernelGGL(verify_pick_kernel<Real>, dim3((unsigned)B), dim3(kVT), 0, st, a);
+            hipLaunchKernelGGL(verify_left_kernel<Real>, left, dim3(kDT), 0, st, a);
+            hipLaunchKernelGGL(verify_pick_kernel<Real>, dim3((unsigned)B), dim3(kDT), 0, st, a);
         }
     });
     RWKV_CHECK_LAUNCH("verify_pick_kernel");
