@@ -16,7 +16,7 @@ constexpr int kVT = kThreads;        // threads of verify_rows_kernel
 constexpr int kPer = 16;             // tokens of a thread
 constexpr int kChunk = kVT * kPer;   // tokens of a workgroup at a time
 // The kernels that draw are short and run once a sequence: what they wait for is their own code, so a thread has four tokens.
-constexpr int kDT = 1024, kFew = kChunk / kDT, kDWaves = kDT / 64;
+constexpr int kDT = 1024, kFew = kChunk / kDT, kDWaves = kDT / 64, kLT = 512;
 constexpr int kSegments = 64;
 constexpr int kMaxDrafts = 64;
 
@@ -43,14 +43,15 @@ struct VerifyArgs {
     Verdict *verdict;                // [B]
 };
 
-// e^d for d <= 0 (anything that is not a number or below -800: 0), to 2^-47 or so: the exponent in 32nds of log2 e from a table, the
+// e^(d / temp) for d <= 0 (0 for anything that is not a number), to 2^-47 or so: the exponent in 32nds of log2 e from a table, the
 // rest by its series (P. T. P. Tang, ACM TOMS 15, 1989).  Half the instructions of exp(), which takes longer than the logits
 // take to come; 2^-47 moves one draw in 10^9.
 struct Exp {
     const double *table;                             // LDS: 2^(i/32)
+    double scale;                                    // 32 log2 e / temp
     __device__ __forceinline__ double operator()(double d) const {
         constexpr double kMagic = 6755399441055744.0;                        // 3 * 2^51: adding it rounds to a whole number
-        const double y = fmax(d, -800.0) * 46.166241308446829;            // 32 log2 e (a d that is no number gives way to -800)
+        const double y = fmax(d * scale, -37000.0);                          // (2^(-37000 / 32) is 0; what is no number gives way to it)
         const double z = y + kMagic, f = y - (z - kMagic);
         const int n = (int)__double_as_longlong(z);
         double p = fma(f, 3.9737099845494161e-11, 9.1725627018246432e-09);          // (ln 2 / 32)^k / k!
@@ -58,8 +59,7 @@ struct Exp {
         p = fma(f, p, 2.3459619820224679e-04);
         p = fma(f, p, 2.1660849392498291e-02);
         p = fma(f, p, 1.0);
-        const double e = ldexp(table[n & 31] * p, n >> 5);
-        return d > -800.0 ? e : 0.0;
+        return ldexp(table[n & 31] * p, n >> 5);
     }
 };
 __constant__ const double kTable[32] = {               // 2^(i/32)
@@ -71,15 +71,13 @@ __constant__ const double kTable[32] = {               // 2^(i/32)
     1.5422108254079408236, 1.5759808451078864865, 1.6104903319492543082, 1.6457554781539648445,
     1.6817928305074290861, 1.7186192981224779156, 1.7562521603732994831, 1.7947090750031071864,
     1.8340080864093424635, 1.8741676341102999013, 1.9152065613971472939, 1.9571441241754002690};
-__device__ __forceinline__ Exp exp_table(double (&table)[32]) {              // (before a barrier)
+__device__ __forceinline__ Exp exp_table(double (&table)[32], double inv_temp) {              // (before a barrier)
     if (threadIdx.x < 32) table[threadIdx.x] = kTable[threadIdx.x];
-    return {table};
+    return {table, inv_temp * 46.166241308446829};
 }
 
 // A logit's weight beside the largest; NaN and -infinity have none, and where the largest is +infinity the others have none.
-__device__ __forceinline__ double weight(Exp e, double x, double max, double inv_temp) {
-    return max == INFINITY ? (x == max ? 1.0 : 0.0) : e((x - max) * inv_temp);
-}
+__device__ __forceinline__ double weight(Exp e, double x, double max) { return max == INFINITY ? (x == max ? 1.0 : 0.0) : e(x - max); }
 
 __device__ __forceinline__ void better(double &x, int &i, double y, int j) {
     if (j >= 0 && (i < 0 || y > x || (y == x && j < i))) { x = y; i = j; }
@@ -134,7 +132,7 @@ template <typename Real, bool GREEDY>
 __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
     __shared__ double s_max[kWaves], red[kWaves], s_exp[32];
     __shared__ int s_first[kWaves];
-    const Exp e = exp_table(s_exp);
+    const Exp e = exp_table(s_exp, a.inv_temp);
     const int64_t targets = a.B * (a.K + 1), at = blockIdx.x, of = at < targets ? a.K + 1 : a.K, row = at < targets ? at : at - targets;
     const Real *x = at < targets ? (const Real *)a.logits + row / of * a.seq + row % of * a.row
                                  : (const Real *)a.draft + row / of * a.draft_seq + row % of * a.draft_row;
@@ -153,10 +151,10 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
 #pragma unroll
             for (int k = 0; k < kPer; ++k) if ((double)v[k] > m) { m = v[k]; first = (int)j + in_chunk<Real>(k); }
         } else {
-            double top = m;
+            Real top = (Real)m;                       // (m is a logit, or -infinity)
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) top = fmax(top, (double)v[k]);
-            s *= weight(e, m, top, a.inv_temp);
+            for (int k = 0; k < kPer; ++k) top = top < v[k] ? v[k] : top;
+            s *= weight(e, m, top);
             m = top;
             if (m == INFINITY) {
 #pragma unroll
@@ -164,7 +162,7 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
             } else {
                 double part[2] = {0.0, 0.0};
 #pragma unroll
-                for (int k = 0; k < kPer; ++k) part[k & 1] += e(((double)v[k] - m) * a.inv_temp);
+                for (int k = 0; k < kPer; ++k) part[k & 1] += e((double)v[k] - m);
                 s += part[0] + part[1];
             }
         }
@@ -184,7 +182,7 @@ __global__ void __launch_bounds__(kVT) verify_rows_kernel(VerifyArgs a) {
         if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
         __syncthreads();
         for (int w = 0; w < kWaves; ++w) m = fmax(m, s_max[w]);
-        double sum[1] = {s * weight(e, own, m, a.inv_temp)};
+        double sum[1] = {s * weight(e, own, m)};
         block_sum(sum, red);
         if (threadIdx.x == 0) *to = {m, sum[0], 0, 0};
     }
@@ -198,9 +196,9 @@ struct Left {
     const Real *x, *y;
     int64_t gone;                    // drafts without a distribution: the one that was refused
     Verdict v;
-    double inv_temp, per_p, per_q;
+    double per_p, per_q;
     Exp e;
-    __device__ Left(const VerifyArgs &a, int64_t b, const Verdict &v_, Exp e_) : v(v_), inv_temp(a.inv_temp), e(e_) {
+    __device__ Left(const VerifyArgs &a, int64_t b, const Verdict &v_, Exp e_) : v(v_), e(e_) {
         x = (const Real *)a.logits + b * a.seq + v.n * a.row;
         y = a.draft && v.left ? (const Real *)a.draft + b * a.draft_seq + v.n * a.draft_row : nullptr;
         gone = v.left ? a.drafts[b * a.K + v.n] : -1;
@@ -209,21 +207,21 @@ struct Left {
     }
     // (px, qx: the logits at j)
     __device__ __forceinline__ double of(double px, double qx, int64_t j) const {
-        const double p = weight(e, px, v.p_max, inv_temp) * per_p;
+        const double p = weight(e, px, v.p_max) * per_p;
         if (!v.left) return p;
-        return fmax(p - (y ? weight(e, qx, v.q_max, inv_temp) * per_q : j == gone ? 1.0 : 0.0), 0.0);
+        return fmax(p - (y ? weight(e, qx, v.q_max) * per_q : j == gone ? 1.0 : 0.0), 0.0);
     }
 };
 
 // A workgroup per sequence and segment; each finds out for itself how many drafts are accepted: rows' segments put together by
 // 16 lanes (64 where there are more), then a thread to a draft.
 template <typename Real>
-__global__ void __launch_bounds__(kDT) verify_left_kernel(VerifyArgs a) {
-    __shared__ double red[kDWaves], s_exp[32], s_max[2 * kMaxDrafts + 1], s_sum[2 * kMaxDrafts + 1];
+__global__ void __launch_bounds__(kLT) verify_left_kernel(VerifyArgs a) {
+    __shared__ double red[kLT / 64], s_exp[32], s_max[2 * kMaxDrafts + 1], s_sum[2 * kMaxDrafts + 1];
     __shared__ Verdict s_v;
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, count = drafts_of(a, b), K = (int)a.K;
-    const Exp e = exp_table(s_exp);
+    const Exp e = exp_table(s_exp, a.inv_temp);
     const RowStat *ps = a.stat + b * (K + 1) * a.segments, *qs = a.stat + (a.B * (K + 1) + b * K) * a.segments;
     // the drafts' own logits, on the way meanwhile
     int64_t d = -1;
@@ -238,14 +236,14 @@ __global__ void __launch_bounds__(kDT) verify_left_kernel(VerifyArgs a) {
     }
     __syncthreads();
     const int lanes = a.segments <= 16 ? 16 : 64, rows = K + 1 + (a.draft ? K : 0);
-    for (int row = tid / lanes; row < (int)round_up(rows, kDT / lanes); row += kDT / lanes) {
+    for (int row = tid / lanes; row < (int)round_up(rows, kLT / lanes); row += kLT / lanes) {
         const int i = tid % lanes;
         const bool in = row < rows && i < a.segments;
         const RowStat *s = (row <= K ? ps + row * a.segments : qs + (row - K - 1) * a.segments) + i;
         const double own = in ? s->max : -INFINITY;
         double max = own, sum = in ? s->sum : 0.0;
         for (int off = lanes / 2; off >= 1; off >>= 1) max = fmax(max, __shfl_xor(max, off, 64));
-        sum *= weight(e, own, max, a.inv_temp);
+        sum *= weight(e, own, max);
         for (int off = lanes / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
         if (in && i == 0) { s_max[row] = max; s_sum[row] = sum; }
     }
@@ -253,8 +251,8 @@ __global__ void __launch_bounds__(kDT) verify_left_kernel(VerifyArgs a) {
     if (tid < 64) {
         bool taken = tid >= count;                    // (beyond the drafts nothing refuses)
         if (d >= 0 && s_sum[tid] > 0) {
-            const double p = weight(e, px, s_max[tid], a.inv_temp) / s_sum[tid];
-            const double q = !a.draft ? 1.0 : s_sum[K + 1 + tid] > 0 ? weight(e, qx, s_max[K + 1 + tid], a.inv_temp) / s_sum[K + 1 + tid] : 0.0;
+            const double p = weight(e, px, s_max[tid]) / s_sum[tid];
+            const double q = !a.draft ? 1.0 : s_sum[K + 1 + tid] > 0 ? weight(e, qx, s_max[K + 1 + tid]) / s_sum[K + 1 + tid] : 0.0;
             taken = u * q < p;
         }
         const unsigned long long refused = __ballot(!taken);
@@ -270,14 +268,15 @@ __global__ void __launch_bounds__(kDT) verify_left_kernel(VerifyArgs a) {
     if (!(v.p_sum > 0)) return;
     if (tid == 0) {                                   // of p itself, for verify_pick_kernel
         const RowStat own = ps[v.n * a.segments + blockIdx.y];
-        a.sums[(a.B + b) * a.segments + blockIdx.y] = own.sum * weight(e, own.max, v.p_max, a.inv_temp) / v.p_sum;
+        a.sums[(a.B + b) * a.segments + blockIdx.y] = own.sum * weight(e, own.max, v.p_max) / v.p_sum;
         if (!v.left) a.sums[b * a.segments + blockIdx.y] = 0.0;
     }
     if (!v.left) return;
     const Left<Real> left(a, b, v, e);
     const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
     double s = 0.0;
-    for (int64_t j = j0 + tid * kFew; j < j1; j += kChunk) {
+#pragma unroll 2
+    for (int64_t j = j0 + tid * kFew; j < j1; j += kLT * kFew) {
         Real x[kFew], y[kFew];
         load_few(x, left.x, j, j1);
         if (left.y) load_few(y, left.y, j, j1);
@@ -289,7 +288,7 @@ __global__ void __launch_bounds__(kDT) verify_left_kernel(VerifyArgs a) {
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-        for (int w = 1; w < kDWaves; ++w) s += red[w];
+        for (int w = 1; w < kLT / 64; ++w) s += red[w];
         a.sums[b * a.segments + blockIdx.y] = s;
     }
 }
@@ -313,7 +312,7 @@ __global__ void __launch_bounds__(kDT) verify_pick_kernel(VerifyArgs a) {
     __shared__ int s_segment, s_left, s_hit[kDWaves], s_last[kDWaves];
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const Exp e = exp_table(s_exp);
+    const Exp e = exp_table(s_exp, a.inv_temp);
     Verdict v = a.verdict[b];
     double own = 0.0, of_p = 0.0;
     if (tid < a.segments) { own = a.sums[b * a.segments + tid]; of_p = a.sums[(a.B + b) * a.segments + tid]; }
@@ -401,7 +400,10 @@ struct VerifyPlan {
     int64_t segment;
     size_t stat_bytes, sum_bytes, verdict_bytes;
     VerifyPlan(int64_t B, int64_t K, int64_t V) {
-        segment = round_up(ceil_div(V, kSegments), kChunk);
+        // no more workgroups than fill the device a few times: each costs as much as 2000 tokens
+        int64_t wanted = ceil_div(4096, B * (2 * K + 1));
+        if (wanted > kSegments) wanted = kSegments;
+        segment = round_up(ceil_div(V, wanted), kChunk);
         segments = (int)ceil_div(V, segment);
         stat_bytes = (size_t)(B * (2 * K + 1) * segments) * sizeof(RowStat);
         sum_bytes = (size_t)(2 * B * segments) * 8;
@@ -450,7 +452,7 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
             hipLaunchKernelGGL(verify_greedy_kernel, dim3((unsigned)B), dim3(kVT), 0, st, a);
         } else {
             hipLaunchKernelGGL((verify_rows_kernel<Real, false>), rows, dim3(kVT), 0, st, a);
-            hipLaunchKernelGGL(verify_left_kernel<Real>, left, dim3(kDT), 0, st, a);
+            hipLaunchKernelGGL(verify_left_kernel<Real>, left, dim3(kLT), 0, st, a);
             hipLaunchKernelGGL(verify_pick_kernel<Real>, dim3((unsigned)B), dim3(kDT), 0, st, a);
         }
     });
