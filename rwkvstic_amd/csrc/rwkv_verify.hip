@@ -3,8 +3,8 @@
 //
 // Each row of logits is cut into segments, at most kSegments of at least kChunk tokens:
 //   verify_rows_kernel  largest logit, and sum of the weights beside it (or first maximum), of every segment of every row
-//   verify_left_kernel  which drafts are accepted; where one is refused, the sums of what is left of its row, segment by segment
-//   verify_pick_kernel  the segment that the drawn token is in, and the token
+//   verify_left_kernel  which drafts are accepted, and the sums of what the next token is drawn from, piece by piece
+//   verify_pick_kernel  the piece that the drawn token is in, and the token
 // Of the logits the first kernel reads everything once; the others read one row of each a sequence (from cache).
 #include "rwkv_types.h"
 
@@ -39,7 +39,8 @@ struct VerifyArgs {
     int segments;
     int64_t segment;                 // tokens of one, a multiple of kChunk
     RowStat *stat;                   // [B][K+1][segments], then [B][K][segments] of the drafts' logits
-    double *sums;                    // [B][segments] of what is left, then [B][segments] of p
+    int64_t piece;                   // a part of a segment: tokens whose weights verify_left_kernel adds up; kSegments at most
+    double *sums;                    // [B][kSegments]
     Verdict *verdict;                // [B]
 };
 
@@ -214,7 +215,7 @@ struct Left {
 };
 
 // A workgroup per sequence and segment; each finds out for itself how many drafts are accepted: rows' segments put together by
-// 16 lanes (64 where there are more), then a thread to a draft.
+// 16 lanes (64 where there are more), then a thread to a draft.  Then the weights of what the token is drawn from, piece by piece.
 template <typename Real>
 __global__ void __launch_bounds__(kLT) verify_left_kernel(VerifyArgs a) {
     __shared__ double red[kLT / 64], s_exp[32], s_max[2 * kMaxDrafts + 1], s_sum[2 * kMaxDrafts + 1];
@@ -266,30 +267,28 @@ __global__ void __launch_bounds__(kLT) verify_left_kernel(VerifyArgs a) {
     __syncthreads();
     const Verdict v = s_v;
     if (!(v.p_sum > 0)) return;
-    if (tid == 0) {                                   // of p itself, for verify_pick_kernel
-        const RowStat own = ps[v.n * a.segments + blockIdx.y];
-        a.sums[(a.B + b) * a.segments + blockIdx.y] = own.sum * weight(e, own.max, v.p_max) / v.p_sum;
-        if (!v.left) a.sums[b * a.segments + blockIdx.y] = 0.0;
-    }
-    if (!v.left) return;
     const Left<Real> left(a, b, v, e);
     const int64_t j0 = blockIdx.y * a.segment, j1 = min(a.V, j0 + a.segment);
-    double s = 0.0;
+    for (int64_t p0 = j0; p0 < j1; p0 += a.piece) {
+        const int64_t p1 = min(j1, p0 + a.piece);
+        double s = 0.0;
 #pragma unroll 2
-    for (int64_t j = j0 + tid * kFew; j < j1; j += kLT * kFew) {
-        Real x[kFew], y[kFew];
-        load_few(x, left.x, j, j1);
-        if (left.y) load_few(y, left.y, j, j1);
+        for (int64_t j = p0 + tid * kFew; j < p1; j += kLT * kFew) {
+            Real x[kFew], y[kFew];
+            load_few(x, left.x, j, p1);
+            if (left.y) load_few(y, left.y, j, p1);
 #pragma unroll
-        for (int k = 0; k < kFew; ++k) s += left.of(x[k], y[k], j + k);
-    }
-    s = wave_sum(s);
-    if ((tid & 63) == 0) red[tid >> 6] = s;
-    __syncthreads();
-    if (tid == 0) {
+            for (int k = 0; k < kFew; ++k) s += left.of(x[k], y[k], j + k);
+        }
+        s = wave_sum(s);
+        __syncthreads();
+        if ((tid & 63) == 0) red[tid >> 6] = s;
+        __syncthreads();
+        if (tid == 0) {
 #pragma unroll
-        for (int w = 1; w < kLT / 64; ++w) s += red[w];
-        a.sums[b * a.segments + blockIdx.y] = s;
+            for (int w = 1; w < kLT / 64; ++w) s += red[w];
+            a.sums[b * kSegments + p0 / a.piece] = s;
+        }
     }
 }
 
@@ -309,32 +308,30 @@ __device__ __forceinline__ double upto(double v, int lane) {                 // 
 template <typename Real>
 __global__ void __launch_bounds__(kDT) verify_pick_kernel(VerifyArgs a) {
     __shared__ double s_wave[kDWaves], s_aim, s_before, s_exp[32];
-    __shared__ int s_segment, s_left, s_hit[kDWaves], s_last[kDWaves];
+    __shared__ int s_piece, s_hit[kDWaves], s_last[kDWaves];
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Exp e = exp_table(s_exp, a.inv_temp);
     Verdict v = a.verdict[b];
-    double own = 0.0, of_p = 0.0;
-    if (tid < a.segments) { own = a.sums[b * a.segments + tid]; of_p = a.sums[(a.B + b) * a.segments + tid]; }
-    const double u = a.u[b * (a.K + 1) + a.K];
+    const int pieces = (int)ceil_div(a.V, a.piece);
+    const double own = tid < pieces ? a.sums[b * kSegments + tid] : 0.0, u = a.u[b * (a.K + 1) + a.K];
+    __syncthreads();
     if (!(v.p_sum > 0)) { answer(a, b, v.n, -1); return; }
     if (tid < 64) {
-        // the segment that passes the aim first, or the last that has anything: of what is left, or of p itself where that is nothing
-        const bool left = __ballot(own > 0.0);
-        if (!left) own = of_p;
+        // the piece that passes the aim first, or the last that has anything; where nothing is left, all of p, which adds up to 1
         const double run = upto(own, lane), aim = u * __shfl(run, 63, 64);
         const unsigned long long any = __ballot(own > 0.0), over = __ballot(own > 0.0 && run > aim);
-        const int at = over ? __ffsll(over) - 1 : 63 - __clzll(any);          // (p has something: its sum is over 0)
-        if (lane == at) { s_segment = at; s_before = run - own; s_aim = aim; s_left = left; }
+        const int at = over ? __ffsll(over) - 1 : any ? 63 - __clzll(any) : 0;
+        if (lane == at) { s_piece = any ? at : -1; s_before = any ? run - own : 0.0; s_aim = any ? aim : u; }
     }
     __syncthreads();
-    v.left = s_left;
+    if (s_piece < 0) v.left = 0;
     const Left<Real> left(a, b, v, e);
-    const int64_t j0 = s_segment * a.segment, j1 = min(a.V, j0 + a.segment);
+    const int64_t j0 = max(s_piece, 0) * a.piece, j1 = s_piece < 0 ? a.V : min(a.V, j0 + a.piece);
     const double aim = s_aim;
     double before = s_before;
     int pick = -1, nearly = -1;                       // rounding can leave no token over the aim: then the segment's last that has weight
-    for (int64_t j = j0; j < j1; j += kChunk) {                         // (one chunk, unless the vocabulary is over kSegments of them)
+    for (int64_t j = j0; j < j1; j += kChunk) {                         // (one chunk, unless the vocabulary is over kSegments of them or nothing was left)
         const int64_t i0 = j + tid * kFew;
         double w[kFew], own = 0.0;
         Real x[kFew], y[kFew];
@@ -397,16 +394,17 @@ __global__ void __launch_bounds__(kVT) verify_greedy_kernel(VerifyArgs a) {
 
 struct VerifyPlan {
     int segments;
-    int64_t segment;
+    int64_t segment, piece;
     size_t stat_bytes, sum_bytes, verdict_bytes;
     VerifyPlan(int64_t B, int64_t K, int64_t V) {
         // no more workgroups than fill the device a few times: each costs as much as 2000 tokens
         int64_t wanted = ceil_div(4096, B * (2 * K + 1));
         if (wanted > kSegments) wanted = kSegments;
-        segment = round_up(ceil_div(V, wanted), kChunk);
+        piece = round_up(ceil_div(V, kSegments), kChunk);
+        segment = round_up(ceil_div(V, wanted), piece);
         segments = (int)ceil_div(V, segment);
         stat_bytes = (size_t)(B * (2 * K + 1) * segments) * sizeof(RowStat);
-        sum_bytes = (size_t)(2 * B * segments) * 8;
+        sum_bytes = (size_t)(B * kSegments) * 8;
         verdict_bytes = (size_t)B * sizeof(Verdict);
     }
     size_t bytes() const { return stat_bytes + sum_bytes + verdict_bytes; }
@@ -441,7 +439,7 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
     uint8_t *ws = (uint8_t *)workspace;
     const bool of_drafts = draft_logits && !greedy && K > 0;
     const VerifyArgs a{B, K, V, logits, logits_seq_stride, logits_row_stride, of_drafts ? draft_logits : nullptr, draft_seq_stride, draft_row_stride,
-                       drafts, lengths, u, 1.0 / temp, tokens, accepted, pl.segments, pl.segment, (RowStat *)ws, (double *)(ws + pl.stat_bytes),
+                       drafts, lengths, u, 1.0 / temp, tokens, accepted, pl.segments, pl.segment, (RowStat *)ws, pl.piece, (double *)(ws + pl.stat_bytes),
                        (Verdict *)(ws + pl.stat_bytes + pl.sum_bytes)};
     const hipStream_t st = (hipStream_t)stream;
     const dim3 rows((unsigned)(B * (K + 1) + (of_drafts ? B * K : 0)), (unsigned)pl.segments), left((unsigned)B, (unsigned)pl.segments);
