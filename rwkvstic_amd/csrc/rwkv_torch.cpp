@@ -35,6 +35,12 @@ struct Entries {
     decltype(&rwkv_mm8_m16_workspace_bytes) mm8_m16_workspace_bytes;
     decltype(&rwkv_mm8_m16) mm8_m16;
     decltype(&rwkv_wkv_f32) wkv_f32;
+    decltype(&rwkv_lora_rows_workspace_bytes) lora_rows_workspace_bytes;
+    decltype(&rwkv_lora_rows) lora_rows;
+    decltype(&rwkv_delta_rule_workspace_bytes) delta_rule_workspace_bytes;
+    decltype(&rwkv_delta_rule) delta_rule;
+    decltype(&rwkv_verify_drafts_workspace_bytes) verify_drafts_workspace_bytes;
+    decltype(&rwkv_verify_drafts) verify_drafts;
 } lib;
 
 void bind(const std::map<std::string, uintptr_t> &at) {
@@ -47,6 +53,9 @@ void bind(const std::map<std::string, uintptr_t> &at) {
     BIND(mm8_packed, rwkv_mm8_packed);
     BIND(mm8_m16_workspace_bytes, rwkv_mm8_m16_workspace_bytes); BIND(mm8_m16, rwkv_mm8_m16);
     BIND(wkv_f32, rwkv_wkv_f32);
+    BIND(lora_rows_workspace_bytes, rwkv_lora_rows_workspace_bytes); BIND(lora_rows, rwkv_lora_rows);
+    BIND(delta_rule_workspace_bytes, rwkv_delta_rule_workspace_bytes); BIND(delta_rule, rwkv_delta_rule);
+    BIND(verify_drafts_workspace_bytes, rwkv_verify_drafts_workspace_bytes); BIND(verify_drafts, rwkv_verify_drafts);
 #undef BIND
 }
 
@@ -242,6 +251,92 @@ pybind11::object wkv_f32(Arg w, Arg u, Arg k, Arg v, Arg aa, Arg bb, Arg pp) {
     return pybind11::cast(y);
 }
 
+// ---- serving operators ---------------------------------------------------------------------------------------------------
+// Results and scratch come from torch's allocator, which gives recorded calls those of the graph that they are recorded into.
+int type_of(const at::Tensor &t) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return RWKV_F32;
+        case at::kDouble: return RWKV_F64;
+        case at::kBFloat16: return RWKV_BF16;
+        case at::kHalf: return RWKV_F16;
+        default: return -1;
+    }
+}
+// a tensor of the current device, of this type and shape
+bool fits(const at::Tensor *t, int device, at::ScalarType dt, at::IntArrayRef shape) {
+    return t && t->is_cuda() && t->get_device() == device && t->scalar_type() == dt && t->sizes() == shape;
+}
+bool fits_whole(const at::Tensor *t, int device, at::ScalarType dt, at::IntArrayRef shape) { return fits(t, device, dt, shape) && t->is_contiguous(); }
+// the distance of the rows of a tensor whose rows are contiguous; -1 where they are not
+int64_t row_stride(const at::Tensor &t) {
+    int64_t n = 1;
+    for (int64_t d = t.dim() - 1; d >= 1; --d) {
+        if (t.size(d) != 1 && t.stride(d) != n) return -1;
+        n *= t.size(d);
+    }
+    return t.size(0) > 1 ? t.stride(0) : n;
+}
+template <typename T = void> T *opt(const at::Tensor *t) { return t ? static_cast<T *>(t->data_ptr()) : nullptr; }
+// an argument that may be None: false if it is something else and no tensor
+bool maybe(Arg a, const at::Tensor *&t) { return a.is_none() || (t = tensor(a)); }
+
+pybind11::object lora_rows(Arg x_, Arg a_, Arg b_, Arg adapter_, Arg scale_, Arg base_, Arg out_) {
+    const at::Tensor *x = tensor(x_), *a = tensor(a_), *b = tensor(b_), *adapter = tensor(adapter_), *scale = nullptr, *base = nullptr, *given = nullptr;
+    if (!x || !a || !b || !maybe(scale_, scale) || !maybe(base_, base) || !maybe(out_, given) || x->dim() != 2 || a->dim() != 3 || b->dim() != 3 || !x->is_cuda()) return pybind11::none();
+    const int dev = current().device_index();
+    const int64_t T = x->size(0), n_in = x->size(1), N = a->size(0), R = a->size(1), n_out = b->size(1);
+    const auto real = x->scalar_type(), low = a->scalar_type();
+    if (T == 0 || (real != at::kFloat && real != at::kDouble) || (low != at::kBFloat16 && low != at::kHalf && low != at::kFloat)) return pybind11::none();
+    if (!fits(x, dev, real, {T, n_in}) || !fits_whole(a, dev, low, {N, R, n_in}) || !fits_whole(b, dev, low, {N, n_out, R}) || !fits_whole(adapter, dev, at::kInt, {T}) ||
+        (scale && !fits_whole(scale, dev, at::kFloat, {N})) || (base && !fits(base, dev, real, {T, n_out})) || (given && !fits(given, dev, real, {T, n_out}))) return pybind11::none();
+    const at::Tensor out = given ? *given : at::empty({T, n_out}, x->options());
+    const int64_t xs = row_stride(*x), bs = base ? row_stride(*base) : 0, os = row_stride(out);
+    if (xs < 0 || bs < 0 || os < 0 || (T > 1 && os < n_out)) return pybind11::none();
+    const at::Tensor ws = bytes(lib.lora_rows_workspace_bytes(T, n_in, n_out, N, R, type_of(*x)), *x);
+    unlocked(lib.lora_rows, T, n_in, n_out, N, R, type_of(*x), opt<const void>(x), xs, type_of(*a), opt<const void>(a), opt<const void>(b), opt<const int32_t>(adapter),
+             opt<const float>(scale), opt<const void>(base), bs, out.data_ptr(), os, ws.data_ptr(), (size_t)ws.numel());
+    return given ? pybind11::reinterpret_borrow<pybind11::object>(out_) : pybind11::cast(out);
+}
+
+pybind11::object delta_rule(Arg q_, Arg k_, Arg v_, Arg g_, Arg beta_, Arg state_, Arg starts_, float scale, Arg out_) {
+    const at::Tensor *q = tensor(q_), *k = tensor(k_), *v = tensor(v_), *g = tensor(g_), *beta = tensor(beta_), *state = tensor(state_), *starts = nullptr, *given = nullptr;
+    if (!q || !k || !v || !state || !maybe(starts_, starts) || !maybe(out_, given) || q->dim() != 3 || v->dim() != 3 || state->dim() != 4 || !q->is_cuda()) return pybind11::none();
+    const int dev = current().device_index();
+    const int64_t T = q->size(0), Hk = q->size(1), dk = q->size(2), Hv = v->size(1), dv = v->size(2), B = state->size(0);
+    const auto dt = q->scalar_type();
+    if (T == 0 || B == 0 || (dt != at::kBFloat16 && dt != at::kHalf && dt != at::kFloat)) return pybind11::none();
+    if (!fits(q, dev, dt, {T, Hk, dk}) || !fits(k, dev, dt, {T, Hk, dk}) || !fits(v, dev, dt, {T, Hv, dv}) || !fits_whole(g, dev, at::kFloat, {T, Hv}) ||
+        !fits_whole(beta, dev, at::kFloat, {T, Hv}) || !fits_whole(state, dev, at::kFloat, {B, Hv, dk, dv}) || (starts ? !fits_whole(starts, dev, at::kInt, {B + 1}) : T % B != 0) ||
+        (given && !fits_whole(given, dev, dt, {T, Hv, dv}))) return pybind11::none();
+    const int64_t qs = row_stride(*q), ks = row_stride(*k), vs = row_stride(*v);
+    if (qs < 0 || ks < 0 || vs < 0) return pybind11::none();
+    const at::Tensor out = given ? *given : at::empty({T, Hv, dv}, v->options());
+    const size_t n = lib.delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv);
+    at::Tensor ws;
+    if (n) ws = bytes(n, *q);
+    unlocked(lib.delta_rule, T, B, Hk, Hv, dk, dv, type_of(*q), opt<const void>(q), qs, opt<const void>(k), ks, opt<const void>(v), vs, opt<const float>(g),
+             opt<const float>(beta), scale, opt<const int32_t>(starts), opt<float>(state), out.data_ptr(), n ? ws.data_ptr() : nullptr, n);
+    return given ? pybind11::reinterpret_borrow<pybind11::object>(out_) : pybind11::cast(out);
+}
+
+pybind11::object verify_drafts(Arg logits_, Arg drafts_, Arg u_, Arg draft_logits_, Arg lengths_, double temp, bool greedy) {
+    const at::Tensor *logits = tensor(logits_), *drafts = tensor(drafts_), *u = nullptr, *of_drafts = nullptr, *lengths = nullptr;
+    if (!logits || !maybe(u_, u) || !maybe(draft_logits_, of_drafts) || !maybe(lengths_, lengths) || logits->dim() != 3 || logits->size(0) == 0 || logits->size(1) == 0 || !logits->is_cuda()) return pybind11::none();
+    const int dev = current().device_index();
+    const int64_t B = logits->size(0), K = logits->size(1) - 1, V = logits->size(2);
+    const auto dt = logits->scalar_type();
+    if ((dt != at::kFloat && dt != at::kDouble) || (!greedy && (!u || !(temp > 0)))) return pybind11::none();
+    if (!fits(logits, dev, dt, {B, K + 1, V}) || !fits_whole(drafts, dev, at::kLong, {B, K}) || (u && !fits_whole(u, dev, at::kFloat, {B, K + 1})) ||
+        (of_drafts && !fits(of_drafts, dev, dt, {B, K, V})) || (lengths && !fits_whole(lengths, dev, at::kInt, {B}))) return pybind11::none();
+    for (const at::Tensor *t : {logits, of_drafts}) if (t && V > 1 && t->stride(2) != 1) return pybind11::none();
+    const at::Tensor tokens = at::empty({B, K + 1}, drafts->options()), accepted = at::empty({B}, drafts->options());
+    const at::Tensor ws = bytes(lib.verify_drafts_workspace_bytes(B, K, V), *logits);
+    unlocked(lib.verify_drafts, B, K, V, type_of(*logits), opt<const void>(logits), logits->stride(0), logits->stride(1), opt<const void>(of_drafts),
+             of_drafts ? of_drafts->stride(0) : 0, of_drafts ? of_drafts->stride(1) : 0, opt<const int64_t>(drafts), opt<const int32_t>(lengths), opt<const float>(u),
+             temp, (int)greedy, ptr<int64_t>(tokens), ptr<int64_t>(accepted), ws.data_ptr(), (size_t)ws.numel());
+    return pybind11::make_tuple(tokens, accepted);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_rwkv_torch, m) {
@@ -250,4 +345,7 @@ PYBIND11_MODULE(_rwkv_torch, m) {
     m.def("mm8_packed", &mm8_packed);
     m.def("mm8_m16", &mm8_m16);
     m.def("wkv_f32", &wkv_f32);
+    m.def("lora_rows", &lora_rows);
+    m.def("delta_rule", &delta_rule);
+    m.def("verify_drafts", &verify_drafts);
 }

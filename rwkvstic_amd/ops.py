@@ -11,6 +11,7 @@ nothing here falls back to torch arithmetic.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Optional, Tuple
 
 import torch
@@ -382,6 +383,11 @@ def _is(t, dtypes, shape, name: str, device=None) -> None:
         raise ValueError(f"{name} must be on {device}")
 
 
+def _elsewhere(t: torch.Tensor):
+    """The device of ``t``, made the current one, where it is another: a launch goes to the current device."""
+    return torch.cuda.device(t.device) if t.device.type == "cuda" and t.device.index != torch.cuda.current_device() else None
+
+
 def _rows(t: torch.Tensor, name: str) -> int:
     """The distance of the rows of ``t [T, ...]``, each of them contiguous."""
     if t.numel() and not t[0].is_contiguous():
@@ -404,6 +410,10 @@ def lora_rows(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.
     and ``b [N, n_out, R]`` bfloat16, float16 or float32 with ``R <= 256`` (adapters of smaller rank are filled up with zeros),
     ``adapter [T]`` int32: a row whose number is outside ``0..N-1`` has no adapter and gets ``base[t]``.  ``scale [N]`` float32;
     without it 1.  ``base``: the shared projection's result, without it 0.  ``out`` may be ``base`` itself."""
+    host = N.host()
+    y = host and host.lora_rows(x, a, b, adapter, scale, base, out)
+    if y is not None:
+        return y
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(a, torch.Tensor) or a.dim() != 3 or not isinstance(b, torch.Tensor) or b.dim() != 3:
         raise ValueError("lora_rows: x must be [T, n_in], a [N, R, n_in], b [N, n_out, R]")
     (T, n_in), (n, R, _), n_out, dev = x.shape, a.shape, b.shape[1], x.device
@@ -421,11 +431,16 @@ def lora_rows(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.
     if T == 0:
         return out
     L, real = N.lib(), _TYPES[x.dtype]
-    ws = _workspace(L.rwkv_lora_rows_workspace_bytes(T, n_in, n_out, n, R, real), dev)
-    N.check(L.rwkv_lora_rows(_stream(), T, n_in, n_out, n, R, real, x.data_ptr(), strides[0], _TYPES[a.dtype], a.data_ptr(), b.data_ptr(),
-                             adapter.data_ptr(), scale.data_ptr() if scale is not None else None,
-                             base.data_ptr() if base is not None else None, strides[1], out.data_ptr(), strides[2], ws.data_ptr(), ws.numel()))
+    with _elsewhere(x) or nullcontext():
+        ws = torch.empty(L.rwkv_lora_rows_workspace_bytes(T, n_in, n_out, n, R, real), dtype=torch.uint8, device=dev)
+        N.check(L.rwkv_lora_rows(_stream(), T, n_in, n_out, n, R, real, x.data_ptr(), strides[0], _TYPES[a.dtype], a.data_ptr(), b.data_ptr(),
+                                 adapter.data_ptr(), scale.data_ptr() if scale is not None else None,
+                                 base.data_ptr() if base is not None else None, strides[1], out.data_ptr(), strides[2], ws.data_ptr(), ws.numel()))
     return out
+
+
+def _default_scale(q) -> float:
+    return q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
 
 
 def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, state: torch.Tensor,
@@ -438,6 +453,11 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     ``state [B, Hv, dk, dv]`` float32, updated in place.  ``starts [B + 1]`` int32 on the device: sequence ``b`` is the rows
     ``starts[b]`` to ``starts[b + 1] - 1``; without it ``T / B`` rows each.  ``scale``: ``dk ** -0.5`` unless given.
     Returns ``o [T, Hv, dv]`` of v's type; rows of no sequence are not written, and an empty sequence keeps its state."""
+    scale = None if scale is None else float(scale)
+    host = N.host()
+    y = host and host.delta_rule(q, k, v, g, beta, state, starts, scale if scale is not None else _default_scale(q), out)
+    if y is not None:
+        return y
     for t, name in ((q, "q"), (v, "v")):
         if not isinstance(t, torch.Tensor) or t.dim() != 3:
             raise ValueError(f"delta_rule: {name} must be [T, heads, channels]")
@@ -459,10 +479,11 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     if T == 0 or B == 0:
         return out
     L = N.lib()
-    ws = _workspace(L.rwkv_delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv), dev)
-    N.check(L.rwkv_delta_rule(_stream(), T, B, Hk, Hv, dk, dv, _TYPES[q.dtype], q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(),
-                              strides[2], g.data_ptr(), beta.data_ptr(), dk ** -0.5 if scale is None else float(scale),
-                              starts.data_ptr() if starts is not None else None, state.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel()))
+    with _elsewhere(q) or nullcontext():
+        ws = torch.empty(L.rwkv_delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv), dtype=torch.uint8, device=dev)
+        N.check(L.rwkv_delta_rule(_stream(), T, B, Hk, Hv, dk, dv, _TYPES[q.dtype], q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(),
+                                  strides[2], g.data_ptr(), beta.data_ptr(), scale if scale is not None else _default_scale(q),
+                                  starts.data_ptr() if starts is not None else None, state.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel()))
     return out
 
 
@@ -477,6 +498,11 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: Optional[torch.
     the lowest index at which the running weight exceeds ``u`` times the whole.  ``draft_logits [B, K, V]`` of logits' type; without them
     the drafts have no distribution of their own (``q(d) = 1``).  ``greedy``: a draft is accepted while it is the first maximum, and the
     token drawn is that maximum.  Row ``b`` of ``tokens`` is the accepted drafts, the token drawn, then -1 (there too, where no logit has weight)."""
+    temp, greedy = float(temp), bool(greedy)
+    host = N.host()
+    y = host and host.verify_drafts(logits, drafts, u, draft_logits, lengths, temp, greedy)
+    if y is not None:
+        return y
     if not isinstance(logits, torch.Tensor) or logits.dim() != 3 or logits.shape[1] < 1:
         raise ValueError("verify_drafts: logits must be [B, K + 1, V]")
     (B, K1, V), dev = logits.shape, logits.device
@@ -499,10 +525,11 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: Optional[torch.
     if B == 0:
         return tokens, accepted
     L = N.lib()
-    ws = _workspace(L.rwkv_verify_drafts_workspace_bytes(B, K1 - 1, V), dev)
     opt = lambda t: t.data_ptr() if t is not None else None
     by = draft_logits.stride() if draft_logits is not None else (0, 0)
-    N.check(L.rwkv_verify_drafts(_stream(), B, K1 - 1, V, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
-                                 opt(draft_logits), by[0], by[1], drafts.data_ptr(), opt(lengths), opt(u), float(temp), 1 if greedy else 0,
-                                 tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel()))
+    with _elsewhere(logits) or nullcontext():
+        ws = torch.empty(L.rwkv_verify_drafts_workspace_bytes(B, K1 - 1, V), dtype=torch.uint8, device=dev)
+        N.check(L.rwkv_verify_drafts(_stream(), B, K1 - 1, V, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), logits.stride(1),
+                                     opt(draft_logits), by[0], by[1], drafts.data_ptr(), opt(lengths), opt(u), temp, 1 if greedy else 0,
+                                     tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), ws.numel()))
     return tokens, accepted
