@@ -17,6 +17,7 @@ namespace {
 constexpr int kDirect = 256;          // most rows whose tiles the wavefronts find for themselves
 constexpr int kWindow = 1024;         // rows sorted together by lora_plan_kernel: a thread each
 constexpr int kSlices = 8;            // most slices of n_in
+constexpr int kFew = 4;               // rows of a tile that are multiplied without the matrix cores, where tiles are found directly
 constexpr int kDownWaves = 8;         // wavefronts of lora_down_kernel: parts of a slice
 
 struct Tile { int first, n, adapter; };          // rows order[first .. first + n - 1]
@@ -290,6 +291,40 @@ __global__ void __launch_bounds__(64 * kDownWaves) lora_down_kernel(LoraArgs p) 
     }
 }
 
+// Few rows of an adapter, float64: on the matrix cores 16 rows would be multiplied all the same, at 64 clocks an instruction.  A thread
+// to an output, whose row of b it reads by itself.  (32 rows of 24 adapters, 2560 to 10240 outputs of rank 64: 17.4 / 13.0 us; float32, whose
+// instructions take 16 clocks: 8.9 / 12.5.)
+template <typename Real, typename Low, bool WIDE>
+__device__ __forceinline__ void up_few(const LoraArgs &p, const Tile &tile, const int *rows, Real *h, int64_t n0, int64_t n1) {
+    for (int at = threadIdx.x; at < tile.n * p.ranks; at += 256) {          // (ranks past the last are 0 in h)
+        const Real *from = (const Real *)p.h + (int64_t)rows[at / p.ranks] * p.ranks + at % p.ranks;
+        Real sum = *from;
+#pragma unroll 4
+        for (int k = 1; k < p.slices; ++k) sum += from[k * p.T * p.ranks];
+        h[at] = sum;
+    }
+    __syncthreads();
+    for (int64_t n = n0 + threadIdx.x; n < n1; n += 256) {
+        const Low *b = (const Low *)p.b + ((int64_t)tile.adapter * p.n_out + n) * p.R;
+        Real base[kFew], acc[kFew] = {};
+#pragma unroll
+        for (int s = 0; s < kFew; ++s) base[s] = p.base && s < tile.n ? ((const Real *)p.base)[(int64_t)rows[s] * p.base_stride + n] : (Real)0;
+#pragma unroll 4
+        for (int k = 0; k < p.R; k += 8) {
+            Eight<Low> bv;
+            load8<WIDE>(bv, b, k, p.R);
+#pragma unroll
+            for (int s = 0; s < kFew; ++s) {
+                if (s >= tile.n) break;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[s] = fma((Real)bv.e[e], h[s * p.ranks + k + e], acc[s]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kFew; ++s) if (s < tile.n) ((Real *)p.out)[(int64_t)rows[s] * p.out_stride + n] = base[s] + acc[s];
+    }
+}
+
 // RB blocks of 32 ranks, NT times 16 rows of the tile: as many as 64 KiB of LDS hold.  An XCD takes the same ranges of outputs
 // for all tiles, and so reads these rows of b once.
 template <typename Real, typename Low, int RB, int NT, int QT, bool WIDE>
@@ -317,6 +352,7 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
         }
         return;
     }
+    if (NT == 1 && sizeof(Real) == 8 && !p.order && tile.n <= kFew) { up_few<Real, Low, WIDE>(p, tile, rows, reinterpret_cast<Real *>(hs), n0, n1); return; }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const Low *b = (const Low *)p.b + (int64_t)tile.adapter * p.n_out * p.R;
     // QT tiles of outputs: lane (j, g) comes out with n + 16 q + 4 g .. + 3 of row j, 64 bytes of a row (128 of float64) to a store
@@ -344,9 +380,14 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
             }
         }
     };
-    Rows now;
+    constexpr int kAll = 4 * 16 * QT;
+    // (everything of the next outputs is on the way while these are multiplied)
+    Rows next;
+    Onto ahead[NT];
     int64_t n = n0 + wave * 16 * QT;
-    load(now, n);
+    load(next, n);
+#pragma unroll
+    for (int s = 0; s < NT; ++s) load_base(ahead[s], s, n);
     for (int at = threadIdx.x; at < n_rows * RB * 8; at += 256) {
         const int r = at / (RB * 8), c = at % (RB * 8) * 4;
         const Real *h = (const Real *)p.h + (int64_t)rows[row0 + r] * p.ranks + c;
@@ -356,13 +397,19 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
         Op::put(hs, NT * 16, RB * 32, r, c, s);
     }
     __syncthreads();
-    while (n < n1) {
-        Onto onto, ahead;
-        load_base(onto, 0, n);
+    for (; n < n1; n += kAll) {
+        const Rows now = next;
+        Onto onto[NT];
+#pragma unroll
+        for (int s = 0; s < NT; ++s) onto[s] = ahead[s];
+        if (n + kAll < n1) {
+            load(next, n + kAll);
+#pragma unroll
+            for (int s = 0; s < NT; ++s) load_base(ahead[s], s, n + kAll);
+        }
 #pragma unroll
         for (int s = 0; s < NT; ++s) {
             if (s * 16 >= n_rows) break;
-            if (s + 1 < NT) load_base(ahead, s + 1, n);
             Vec acc[QT];
 #pragma unroll
             for (int q = 0; q < QT; ++q) acc[q] = Vec{0, 0, 0, 0};
@@ -372,22 +419,18 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
 #pragma unroll
                 for (int q = 0; q < QT; ++q) Op::add(acc[q], now.v[q][k], r);
             }
-            if (s * 16 + i < n_rows) {
-                Real *to = out + (int64_t)rows[row0 + s * 16 + i] * p.out_stride + n + 4 * g;
+            if (s * 16 + i >= n_rows) continue;
+            Real *to = out + (int64_t)rows[row0 + s * 16 + i] * p.out_stride + n + 4 * g;
 #pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                    acc[q] += onto.v[q];
-                    if (WIDE) { if (n + 4 * g + 16 * q < n1) *reinterpret_cast<Vec *>(to + 16 * q) = acc[q]; }
-                    else {
+            for (int q = 0; q < QT; ++q) {
+                acc[q] += onto[s].v[q];
+                if (WIDE) { if (n + 4 * g + 16 * q < n1) *reinterpret_cast<Vec *>(to + 16 * q) = acc[q]; }
+                else {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) if (n + 4 * g + 16 * q + c < n1) to[16 * q + c] = acc[q][c];
-                    }
+                    for (int c = 0; c < 4; ++c) if (n + 4 * g + 16 * q + c < n1) to[16 * q + c] = acc[q][c];
                 }
             }
-            onto = ahead;
         }
-        n += 4 * 16 * QT;
-        if (n < n1) load(now, n);
     }
 }
 
@@ -395,7 +438,7 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
 struct LoraPlan {
     bool direct;
     int windows, slots;                   // tiles are looked for in windows * slots places
-    int group, groups, ranks;             // tiles of 16 ranks to a wavefront of lora_down_kernel, and wavefronts
+    int group, groups, ranks;             // tiles of 16 ranks to a wavefront of lora_down_kernel, and wavefronts; ranks: 32, 64, 128 or 256
     int slices, steps, range, chunks;
     size_t h_bytes, order_bytes, tile_bytes;
     LoraPlan(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real) {
@@ -405,13 +448,14 @@ struct LoraPlan {
         group = R <= 32 ? 2 : R <= 64 ? 4 : 8;
         groups = (int)ceil_div(R, group * 16);
         ranks = group * groups * 16;
+        // workgroups for the whole device, while a wavefront has terms left to do
         const int64_t blocks = ceil_div(n_in, 32), tiles = direct ? T : ceil_div(T, 16);
         int64_t s = 1;
-        while (s < kSlices && s * tiles < (direct ? 256 : 512) && blocks > s * kDownWaves) s *= 2;
+        while (s < kSlices && s * tiles < (direct ? 512 : 1024) && blocks > s * kDownWaves) s *= 2;
         steps = (int)ceil_div(blocks, kDownWaves * s);
         slices = (int)ceil_div(blocks, kDownWaves * steps);
-        const int64_t wanted = ceil_div(direct ? 2048 : 1024, direct ? T : ceil_div(T, 64));
-        range = (int)round_up(ceil_div(n_out, wanted), direct || real == RWKV_F64 ? 128 : 256);
+        const int64_t wanted = ceil_div(direct || real == RWKV_F64 ? 2048 : 1024, direct ? T : ceil_div(T, 64));
+        range = (int)round_up(ceil_div(n_out, wanted), direct ? 256 : 128);
         chunks = (int)ceil_div(n_out, range);
         if (chunks > 8) chunks = (int)round_up(chunks, 8);
         h_bytes = round_up((size_t)slices * T * ranks * type_bytes(real), 256);
@@ -441,11 +485,11 @@ void launch(hipStream_t st, const LoraPlan &pl, const LoraArgs &p) {
         hipLaunchKernelGGL(pl.direct ? one : many, up, dim3(256), (size_t)rows * Op::row_bytes(pl.ranks), st, p);
     };
     constexpr int k128 = sizeof(Real) == 4 ? 4 : 2, k256 = k128 / 2;            // rows in LDS, by ranks
-    constexpr int kWide = sizeof(Real) == 4 ? 4 : 2;                            // tiles of outputs to a wavefront: 256 bytes of a row
-    if (pl.ranks == 32) go_up(lora_up_kernel<Real, Low, 1, 1, 2, WIDE>, lora_up_kernel<Real, Low, 1, 4, kWide, WIDE>, 4);
-    else if (pl.ranks == 64) go_up(lora_up_kernel<Real, Low, 2, 1, 2, WIDE>, lora_up_kernel<Real, Low, 2, 4, kWide, WIDE>, 4);
-    else if (pl.ranks == 128) go_up(lora_up_kernel<Real, Low, 4, 1, 2, WIDE>, lora_up_kernel<Real, Low, 4, k128, kWide, WIDE>, k128);
-    else go_up(lora_up_kernel<Real, Low, 8, 1, 2, WIDE>, lora_up_kernel<Real, Low, 8, k256, 2, WIDE>, k256);
+    constexpr int kWide = sizeof(Real) == 4 ? 2 : 1;                            // tiles of outputs to a wavefront: 128 bytes of a row
+    if (pl.ranks == 32) go_up(lora_up_kernel<Real, Low, 1, 1, kWide, WIDE>, lora_up_kernel<Real, Low, 1, 4, kWide, WIDE>, 4);
+    else if (pl.ranks == 64) go_up(lora_up_kernel<Real, Low, 2, 1, kWide, WIDE>, lora_up_kernel<Real, Low, 2, 4, kWide, WIDE>, 4);
+    else if (pl.ranks == 128) go_up(lora_up_kernel<Real, Low, 4, 1, kWide, WIDE>, lora_up_kernel<Real, Low, 4, k128, kWide, WIDE>, k128);
+    else go_up(lora_up_kernel<Real, Low, 8, 1, kWide, WIDE>, lora_up_kernel<Real, Low, 8, k256, kWide, WIDE>, k256);
 }
 
 }  // namespace
