@@ -44,7 +44,8 @@ def _near(got, want, bound, half):
     (1, 64, 64, 1, 1, "shuffled"), (1, 2560, 768, 4, 16, "shuffled"), (5, 33, 17, 3, 5, "shuffled"), (16, 256, 320, 1, 64, "segments"),
     (31, 1000, 999, 40, 8, "shuffled"), (64, 512, 512, 7, 33, "shuffled"), (65, 130, 260, 2, 17, "shuffled"), (200, 192, 1024, 3, 128, "segments"),
     (333, 768, 500, 16, 32, "shuffled"), (77, 96, 129, 64, 256, "shuffled"), (1030, 128, 64, 5, 4, "segments"), (129, 3, 2, 2, 2, "shuffled"),
-    (40, 5000, 72, 2, 24, "segments"), (600, 80, 48, 300, 9, "shuffled")])
+    (40, 5000, 72, 2, 24, "segments"), (600, 80, 48, 300, 9, "shuffled"), (256, 64, 40, 9, 12, "shuffled"), (257, 64, 40, 9, 12, "shuffled"),
+    (1024, 32, 36, 1500, 4, "shuffled"), (1025, 40, 24, 1, 40, "segments"), (2100, 24, 16, 1200, 3, "segments"), (6, 2048, 2048, 1, 64, "segments")])
 def test_adapters_of_many_requests(ops, real, low, T, n_in, n_out, N, R, order):
     c = _adapters(T, n_in, n_out, N, R, real, low, T + n_in + R, order)
     print(f"adapters {T} {n_in} {n_out} {N} {R} {order} {real} {low}", flush=True)
@@ -82,7 +83,7 @@ def test_adapters_of_rows_that_lie_apart(ops, real, T):
     _near(ops.lora_rows(one, d["a"], d["b"], d["adapter"]), want, bound, HALF[real])
 
 
-@pytest.mark.parametrize("T", [4, 40, 150])
+@pytest.mark.parametrize("T", [4, 40, 150, 400])
 def test_rows_without_an_adapter_and_rows_that_are_not_numbers(ops, T):
     c = _adapters(T, 256, 192, 3, 16, torch.float32, torch.bfloat16, 2)
     c["adapter"][0], c["adapter"][1], c["adapter"][2], c["adapter"][3] = 3, -7, 1, 2 ** 31 - 1
@@ -254,7 +255,7 @@ def _verify(ops, logits, drafts, u, **kw):
 
 
 @pytest.mark.parametrize("real", [torch.float64, torch.float32])
-@pytest.mark.parametrize("B,K,V", [(1, 0, 1), (1, 4, 50277), (3, 2, 5), (9, 5, 1000), (2, 64, 777), (40, 3, 4097), (5, 8, 65536), (130, 1, 63), (1, 1, 200001)])
+@pytest.mark.parametrize("B,K,V", [(1, 0, 1), (1, 4, 50277), (3, 2, 5), (9, 5, 1000), (2, 64, 777), (40, 3, 4097), (5, 8, 65536), (130, 1, 63), (1, 1, 200001), (150, 13, 9000), (2, 2, 300000)])
 def test_drafts_by_sampling(ops, real, B, K, V):
     print(f"verify {B} {K} {V} {real}", flush=True)
     g = torch.Generator().manual_seed(V)
@@ -294,6 +295,16 @@ def test_drafts_at_the_edges(ops, real):
     _verify(ops, logits, drafts, u, greedy=True)
     u[11], u[12] = -1.0, 2.0
     _verify(ops, logits, drafts, u, draft_logits=draft)
+
+
+@pytest.mark.parametrize("V", [9, 5000, 270000])
+def test_nothing_left_of_the_distribution(ops, V):
+    """Target and drafter agree to the last bit and the random number refuses all the same (it is 1): the token is drawn from p."""
+    logits, drafts, u, draft = P.verify_inputs(5, 2, V, torch.float64, V)
+    draft = logits[:, :2].clone()
+    u[:, :2] = 1.0
+    tokens = _verify(ops, logits, drafts, u, draft_logits=draft)[0]
+    assert bool((tokens[:, 0] >= 0).all()) and bool((tokens[:, 1:] == -1).all())
 
 
 @pytest.mark.parametrize("greedy", [False, True])
