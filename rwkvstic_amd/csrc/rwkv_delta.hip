@@ -7,6 +7,10 @@
 //   O = scale e^G Q S + P U,  P_ij = scale e^(G_i - G_j) q_i.k_j up to the diagonal,  S <- e^G_64 S + K^T (e^(G_64 - G) U).
 //   delta_within_kernel   T and P of every chunk, all at once
 //   delta_chunks_kernel   chunk after chunk, a wavefront to 16 columns of the state
+// Where that leaves most of the device idle (few sequences and heads), a sequence is cut into segments: what a segment makes of the
+// state before it, S -> M S + N, is computed for all of them side by side (the chunks from 0, and from the identity without values), then
+//   delta_join_kernel     puts the segments together, for the state in front of each,
+// and the segments are gone through once more from there, for their outputs.
 // Both on the matrix cores with float32 sums; G and its differences are float64, as a decay is the exponential of a difference of sums.
 // A float32 operand goes into the bfloat16 matrix instructions as the sum of three bfloat16 values, its 24 bits cut in three
 // (planes); of the products of planes those below 2^-24 are left out: three products with bfloat16 keys, six of two float32
@@ -29,6 +33,9 @@ struct DeltaArgs {
     const int32_t *starts;
     float *state;
     void *o;
+    int segments;                         // of a sequence, as many as its chunks allow
+    float *ends, *fronts;                 // with segments: [B][Hv][segments][dk][across] N and M; [B][Hv][segments][dk][dv] states in front
+    int values, across;                   // columns of N, dv filled up to 64s, and of N and M, with dk filled up to the kernel's tiles
 };
 
 // First row and number of rows of sequence b, cut to the rows there are.
@@ -37,6 +44,29 @@ __device__ __forceinline__ void rows_of(const DeltaArgs &a, int64_t b, int64_t &
     const int64_t lo = a.starts[b], hi = a.starts[b + 1];
     first = min(max(lo, (int64_t)0), a.T);
     n = max(min(hi, a.T) - first, (int64_t)0);
+}
+
+// The sequence at a place of the order in which they are begun: the longest first, so that none of them is begun when the others are
+// nearly done; as they come where there are more than a wavefront's lanes.  (8192 rows of seven ragged sequences, 32 heads of
+// 128 x 128, bfloat16: 248 us against 270)
+__device__ __forceinline__ int64_t begun(const DeltaArgs &a, int64_t at) {
+    if (!a.starts || a.B > 64) return at;
+    const int lane = threadIdx.x & 63;
+    int64_t first, n = -1;
+    if (lane < a.B) rows_of(a, lane, first, n);
+    int before = 0;
+    for (int other = 0; other < a.B; ++other) {
+        const int m = __builtin_amdgcn_readlane((int)n, other);
+        before += m > (int)n || (m == (int)n && other < lane);
+    }
+    return __ffsll((long long)__ballot(before == (int)at)) - 1;
+}
+
+// A segment of a sequence of n rows: its first chunk, and how many; none where the sequence has fewer.
+__device__ __forceinline__ int64_t segment_of(const DeltaArgs &a, int64_t n, int segment, int64_t &begin) {
+    const int64_t chunks = (n + 63) / 64, each = (chunks + a.segments - 1) / a.segments;
+    begin = segment * each;
+    return max(min(each, chunks - begin), (int64_t)0);
 }
 
 // Sum over the 16 lanes of a DPP row, in every one of them.
@@ -251,8 +281,8 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
     __shared__ __align__(16) float s_A[kChunk][kChunk + 4], s_X[4][16][20];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
     const int h = blockIdx.y, hk = h / a.share;
-    // the last sequence whose places begin here or before
     const int64_t place = blockIdx.x;
+    // the last sequence whose places begin here or before
     int64_t b = -1;
     for (int64_t b0 = 0; b0 < a.B; b0 += 64) {
         int64_t first = 0, n = 0;
@@ -293,14 +323,21 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
         const int row = min(16 * m + i, live - 1), column = min(16 * (block - block_of(m, 0)) + i, live - 1);
         kr[x] = keys + row * a.k_stride; qr[x] = queries + row * a.q_stride; kc[x] = keys + column * a.k_stride;
     }
-#pragma unroll 2
-    for (int k = E * g; k < a.dk + E * g; k += 4 * E) {
+    auto terms = [&](int k, auto whole) {                 // (whole: none of the block's 4 E terms is behind the last)
+        auto some = [&](const T *row) {
+            if constexpr (decltype(whole)::value && WIDE) return *reinterpret_cast<const typename Some<T, E>::type *>(row + k);
+            else return take<E, WIDE>(row, k, a.dk);
+        };
         typename Some<T, E>::type l[kMost], r[kMost], q[kMost];
 #pragma unroll
-        for (int x = 0; x < kMost; ++x) { l[x] = take<E, WIDE>(kc[x], k, a.dk); r[x] = take<E, WIDE>(kr[x], k, a.dk); q[x] = take<E, WIDE>(qr[x], k, a.dk); }
+        for (int x = 0; x < kMost; ++x) { l[x] = some(kc[x]); r[x] = some(kr[x]); q[x] = some(qr[x]); }
 #pragma unroll
         for (int x = 0; x < kMost; ++x) { kk[x] = dot_step(l[x], r[x], kk[x]); qk[x] = dot_step(l[x], q[x], qk[x]); }
-    }
+    };
+    int k = 0;
+#pragma unroll 2
+    for (; k + 4 * E <= a.dk; k += 4 * E) terms(k + E * g, std::true_type{});
+    if (k < a.dk) terms(k + E * g, std::false_type{});
     __syncthreads();
     // A into LDS, P out
 #pragma unroll
@@ -378,23 +415,33 @@ template <typename T, int NK> struct Chunks {
     static constexpr int kRows = NK >= 8 ? 4 : 2, kPieces = NK * 2 * (kChunk / kRows) / kThreads;          // rows of a piece of K or Q, pieces of a thread
 };
 
-template <typename T, int NK, bool WIDE>
-__global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
+// SUMMARY: a segment's N (groups of columns of values, from 0 or, the first segment, from the state) and M (groups behind them, from
+// the identity, of no values); no outputs.
+template <typename T, int NK, bool WIDE, bool SUMMARY>
+__global__ void __launch_bounds__(kThreads, NK <= 4 ? 2 : 1) delta_chunks_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
     using C = Chunks<T, NK>;
     using V8 = typename Some<T, 8>::type;
     using V4 = typename Some<T, 4>::type;
     constexpr int kIn = C::kIn, kRows = C::kRows, kPieces = C::kPieces, kAcross = kChunk / kRows;
     extern __shared__ __align__(16) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
-    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / a.share;
-    const int64_t b = blockIdx.x / groups / a.Hv;
-    const int col0 = (int)(blockIdx.x % groups) * 64, col = col0 + wave * 16 + i;
+    const int places = SUMMARY ? a.across / 64 : groups;
+    const uint32_t unit = blockIdx.x / places, heads = (uint32_t)(a.B * a.Hv);          // (segments last: each compute unit gets some of all)
+    const int segment = (int)(unit / heads), place = (int)(blockIdx.x % places), h = (int)(unit % a.Hv), hk = h / a.share;
+    const int64_t b = begun(a, unit % heads / a.Hv), bh = b * a.Hv + h;
+    const bool identity = SUMMARY && place >= groups;
+    const int col0 = (place - (identity ? groups : 0)) * 64, col = col0 + wave * 16 + i;
     const bool in = col < a.dv;
-    int64_t first, n;
+    int64_t first, n, begin;
     rows_of(a, b, first, n);
     if (n <= 0) return;
+    const int64_t chunks = segment_of(a, n, segment, begin);
+    const bool at_end = (begin + chunks) * kChunk >= n;
+    if (chunks <= 0 || (SUMMARY && (at_end || (identity && segment == 0)))) return;
+    const f32x4 *slot = slots + ((place_of(first, b) + begin) * a.Hv + h) * kUnits;
+    first += begin * kChunk;
+    n = min(n - begin * kChunk, chunks * kChunk);
     const int64_t end = (n - 1) / kChunk * kChunk;       // the last chunk
-    const f32x4 *slot = slots + (place_of(first, b) * a.Hv + h) * kUnits;
     // Offsets within a chunk fit 32 bits (the host has looked).  Rows behind the last are the last again, columns the first: T's
     // columns are 0 there, and what comes of them is not written.  Behind the last chunk it is fetched again.
     auto piece = [&](V8 *to, const T *from, int64_t stride, int64_t done, int count, int r, int c, int channels) {
@@ -416,7 +463,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
 #pragma unroll
         for (int m = 0; m < kPieces; ++m) {
             piece(keys_next[m], (const T *)a.k + (int64_t)hk * a.dk, a.k_stride, done, kRows, r, c0 + m * (kThreads / kAcross), a.dk);
-            piece(queries_next[m], (const T *)a.q + (int64_t)hk * a.dk, a.q_stride, done, kRows, r, c0 + m * (kThreads / kAcross), a.dk);
+            if (!SUMMARY) piece(queries_next[m], (const T *)a.q + (int64_t)hk * a.dk, a.q_stride, done, kRows, r, c0 + m * (kThreads / kAcross), a.dk);
         }
     };
     auto fetch_rest = [&](int64_t done) {
@@ -424,7 +471,8 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
 #pragma unroll
         for (int m = 0; m < kBlocks / 2; ++m) blocks_next[m] = units[m * kThreads + tid];
         decay_next = reinterpret_cast<const float *>(units + kUnitG)[tid % (2 * kChunk)];
-        piece(values_next, (const T *)a.v + (int64_t)h * a.dv + col0, a.v_stride, done, 2, r_values, c_values, a.dv - col0);
+        if (identity) values_next[0] = values_next[1] = V8((T)0.f);
+        else piece(values_next, (const T *)a.v + (int64_t)h * a.dv + col0, a.v_stride, done, 2, r_values, c_values, a.dv - col0);
     };
     auto cut = [&](const V8 &x, int c) { return planes_of(WIDE && 8 * c >= a.dk ? V8((T)0.f) : x); };
     auto put_rows = [&](const V8 (&x)[kPieces][kRows], int of) {
@@ -508,12 +556,20 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
     fetch_rows(0);
     fetch_rest(0);
     for (int at = tid; at < 2 * kPairs * 3 * 64; at += kThreads) reinterpret_cast<u32x4 *>(lds + C::kPairsAt)[at] = u32x4{0, 0, 0, 0};      // (pairs' blocks above the diagonal)
-    float *state = a.state + (b * a.Hv + h) * a.dk * a.dv + (in ? col : 0);
+    float *const state = a.state + bh * a.dk * a.dv, *const front = a.fronts + (bh * a.segments + segment) * a.dk * a.dv;
+    const float *const from_state = SUMMARY || (segment == 0 && at_end) ? state : front;          // (a sequence of one segment has no summary)
     f32x4 S[NK];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; S[k][v] = row < a.dk ? state[(int64_t)row * a.dv] : 0.f; }
+        for (int v = 0; v < 4; ++v) {
+            const int row = 16 * k + 4 * g + v;
+            if (SUMMARY && (identity || segment)) S[k][v] = identity && row == col && row < a.dk ? 1.f : 0.f;
+            else {
+                S[k][v] = row < a.dk ? from_state[(int64_t)row * a.dv + (in ? col : 0)] : 0.f;
+                if (SUMMARY && in && row < a.dk) front[(int64_t)row * a.dv + col] = S[k][v];          // (the last segment writes the state while the first reads it)
+            }
+        }
     __syncthreads();
     auto keep = [&] {
 #pragma unroll
@@ -522,7 +578,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
             for (int y = 0; y < kRows; ++y) keys_now[m][y] = keys_next[m][y];
     };
     put_rows(keys_next, 0);
-    put_rows(queries_next, 1);
+    if (!SUMMARY) put_rows(queries_next, 1);
     put_rest();
     keep();
     fetch_rows(min((int64_t)kChunk, end));
@@ -539,14 +595,17 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
             const Planes<3> s = planes<3>(S[2 * k], S[2 * k + 1]);
-            const Planes<kIn> keys[4] = {rows(0, 0, k), rows(0, 1, k), rows(0, 2, k), rows(0, 3, k)}, queries[4] = {rows(1, 0, k), rows(1, 1, k), rows(1, 2, k), rows(1, 3, k)};
+            const Planes<kIn> keys[4] = {rows(0, 0, k), rows(0, 1, k), rows(0, 2, k), rows(0, 3, k)};
             add_planes(kS, keys, s);
-            add_planes<true>(O, queries, s);
+            if constexpr (!SUMMARY) {
+                const Planes<kIn> queries[4] = {rows(1, 0, k), rows(1, 1, k), rows(1, 2, k), rows(1, 3, k)};
+                add_planes<true>(O, queries, s);
+            }
         }
         __syncthreads();
         // U and O; K and Q of the next chunk into LDS
         put_rows(keys_next, 0);
-        put_rows(queries_next, 1);
+        if (!SUMMARY) put_rows(queries_next, 1);
         keep();
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -566,7 +625,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
             acc[2] = two[0]; acc[3] = two[1];
         };
         below(std::false_type{}, U, 0, R);
-        below(std::true_type{}, O, 1, U);
+        if constexpr (!SUMMARY) below(std::true_type{}, O, 1, U);
         const float last = decays[kChunk - 1];
 #pragma unroll
         for (int m = 0; m < 4; ++m) U[m] *= *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
@@ -574,7 +633,7 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
         // S; T, P and V of the next chunk into LDS, K and Q of the one after that on the way (behind the stores, which are waited for with them)
         put_rest();
         T *const o = (T *)a.o + ((first + done) * a.Hv + h) * a.dv;
-        const int live = (int)min((int64_t)kChunk, n - done), from = col0 + wave * 16 + 4 * g;
+        const int live = SUMMARY ? 0 : (int)min((int64_t)kChunk, n - done), from = col0 + wave * 16 + 4 * g;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             if (16 * m + i >= live) break;
@@ -599,11 +658,82 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_kernel(DeltaArgs a, con
         }
         __syncthreads();
     }
-    if (in)
+    float *const ends = a.ends + (bh * a.segments + segment) * a.dk * a.across + (identity ? groups * 64 : 0);
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+    for (int k = 0; k < NK; ++k)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; if (row < a.dk) state[(int64_t)row * a.dv] = S[k][v]; }
+        for (int v = 0; v < 4; ++v) {
+            const int row = 16 * k + 4 * g + v;
+            if (row >= a.dk) continue;
+            if (SUMMARY) { if (identity ? col < NK * 16 : true) ends[(int64_t)row * a.across + col] = S[k][v]; }
+            else if (at_end && in) state[(int64_t)row * a.dv + col] = S[k][v];
+        }
+}
+
+// The state in front of each segment but the first: X_1 = N_0, X_(s+1) = N_s + M_s X_s, with float32 instructions.  A workgroup to 16
+// columns, a wavefront to NK / 4 tiles of 16 rows; X goes round through LDS as the accumulators hold it, which is how the products
+// take it: lane (i, g) has rows 4 g .. + 3 of column i.  Each piece of the next M is asked for as soon as this one's is used.
+template <int NK>
+__global__ void __launch_bounds__(kThreads) delta_join_kernel(DeltaArgs a, int columns) {
+    constexpr int kTiles = NK / 4;
+    __shared__ f32x4 s_X[2][NK * 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int64_t bh = blockIdx.x / columns;
+    const int col = (int)(blockIdx.x % columns) * 16 + i;
+    int64_t first, n;
+    rows_of(a, bh / a.Hv, first, n);
+    const int64_t chunks = (n + kChunk - 1) / kChunk, each = max((chunks + a.segments - 1) / a.segments, (int64_t)1);
+    const int last = (int)((chunks + each - 1) / each) - 1;            // (its state in front is the last one)
+    f32x4 M[kTiles][NK], N[kTiles];
+    auto left = [&](int segment, int t, int k) {
+        const float *row = a.ends + ((bh * a.segments + segment) * a.dk + min(16 * (wave * kTiles + t) + i, a.dk - 1)) * a.across + a.values;
+        return *reinterpret_cast<const f32x4 *>(row + 16 * k + 4 * g);
+    };
+    auto added = [&](int segment, int t) {
+        f32x4 to;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int row = 16 * (wave * kTiles + t) + 4 * g + v;
+            to[v] = row < a.dk ? a.ends[((bh * a.segments + segment) * a.dk + row) * a.across + col] : 0.f;
+        }
+        return to;
+    };
+    if (last < 1) return;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+        N[t] = added(0, t);
+        if (last > 1) {
+#pragma unroll
+            for (int k = 0; k < NK; ++k) M[t][k] = left(1, t, k);
+        }
+    }
+    for (int segment = 0; segment < last; ++segment) {
+        const int next = min(segment + 1, last - 1);
+        const f32x4 *X = s_X[segment & 1];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            f32x4 sum[2] = {N[t], f32x4{0, 0, 0, 0}};
+            N[t] = added(next, t);
+            if (segment) {
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {
+                    const f32x4 x = X[k * 64 + lane], m = M[t][k];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) sum[k & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[v], x[v], sum[k & 1], 0, 0, 0);
+                    M[t][k] = left(next, t, k);
+                }
+            }
+            sum[0] += sum[1];
+            const int row = 16 * (wave * kTiles + t) + 4 * g;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                if (row + v >= a.dk) sum[0][v] = 0.f;          // (its row of M is the last one's)
+                else if (col < a.dv) a.fronts[((bh * a.segments + segment + 1) * a.dk + row + v) * a.dv + col] = sum[0][v];
+            }
+            s_X[~segment & 1][(wave * kTiles + t) * 64 + lane] = sum[0];
+        }
+        __syncthreads();
+    }
 }
 
 // The same with float32 operands and instructions, where K, Q and K^T in planes are more than LDS holds.
@@ -695,13 +825,37 @@ __global__ void __launch_bounds__(256) delta_chunks_f32_kernel(DeltaArgs a, cons
 constexpr int kManyRows = 48;
 bool in_chunks(int64_t T, int64_t B) { return T >= kManyRows * B; }
 
+// How the chunks are gone through; the same for a call's workspace and its launches.
+struct DeltaPlan {
+    bool chunks;
+    int tiles, groups, across, segments;             // tiles of 16 key channels, groups of 64 value channels
+    size_t slot_bytes, end_bytes, front_bytes;
+    DeltaPlan(int64_t T, int64_t B, int64_t Hv, int64_t dk, int64_t dv) {
+        chunks = in_chunks(T, B);
+        tiles = dk <= 64 ? 4 : dk <= 128 ? 8 : 16;
+        groups = (int)ceil_div(dv, 64);
+        across = 64 * groups + 16 * tiles;
+        // As many segments as leave a compute unit to every workgroup and four chunks to a segment; of two nothing would be gained.
+        // One sequence of 1024 rows, 40 heads of 64 x 64, float32: 88 us in one piece, 28 (N and M) + 6 (joined) + 29 (outputs) in
+        // four; of 2048 rows, 32 heads of 128 x 128, bfloat16: 148 in one, 56 + 10 + 64 in three (float16: 209, 69 + 10 + 87).
+        const int64_t each = B * Hv, all = across / 64;
+        int64_t s = T / B / (4 * kChunk);
+        while (s > 2 && (each * (groups + (s - 2) * all) > 256 || each * groups * s > 256)) --s;
+        segments = (int)(s > 2 ? s < 16 ? s : 16 : 1);
+        slot_bytes = (size_t)((T / kChunk + B) * Hv) * kUnits * 16;
+        end_bytes = segments > 1 ? (size_t)(each * segments * dk * across) * 4 : 0;
+        front_bytes = segments > 1 ? (size_t)(each * segments * dk * dv) * 4 : 0;
+    }
+    size_t bytes() const { return chunks ? slot_bytes + end_bytes + front_bytes : 0; }
+};
+
 template <typename F> int by_channels(int dk, F &&fn) {
     return dk <= 32 ? fn(std::integral_constant<int, 2>{}) : dk <= 64 ? fn(std::integral_constant<int, 4>{}) : dk <= 128 ? fn(std::integral_constant<int, 8>{}) : fn(std::integral_constant<int, 16>{});
 }
 
 template <typename T, bool WIDE>
-int launch(hipStream_t st, const DeltaArgs &a, f32x4 *slots) {
-    if (!in_chunks(a.T, a.B)) {
+int launch(hipStream_t st, const DeltaArgs &a, const DeltaPlan &pl, f32x4 *slots) {
+    if (!pl.chunks) {
         const int tiles = (int)ceil_div(a.dv, 16);
         return by_channels(a.dk, [&](auto nr) {
             hipLaunchKernelGGL((delta_steps_kernel<T, decltype(nr)::value, WIDE>), dim3((unsigned)ceil_div(a.B * a.Hv * tiles, 4)), dim3(256), 0, st, a, tiles);
@@ -713,13 +867,25 @@ int launch(hipStream_t st, const DeltaArgs &a, f32x4 *slots) {
     RWKV_CHECK_LAUNCH("delta_within_kernel");
     return by_channels(a.dk, [&](auto nk) {
         constexpr int NK = decltype(nk)::value < 4 ? 4 : decltype(nk)::value;
-        constexpr bool kInPlanes = Chunks<T, NK>::kBytes <= 160 * 1024;
-        constexpr size_t bytes = kInPlanes ? Chunks<T, NK>::kBytes : 2 * kChunk * (NK * 16 + 4) * 4;
-        constexpr auto kernel = [] { if constexpr (kInPlanes) return &delta_chunks_kernel<T, NK, WIDE>; else return &delta_chunks_f32_kernel<T, NK, WIDE>; }();
-        if (const int rc = allow_lds<kernel>(bytes)) return rc;
-        const int groups = (int)ceil_div(a.dv, 64);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(a.B * a.Hv * groups)), dim3(kThreads), bytes, st, a, slots, groups);
-        RWKV_CHECK_LAUNCH("delta_chunks_kernel");
+        const unsigned heads = (unsigned)(a.B * a.Hv);
+        if constexpr (Chunks<T, NK>::kBytes <= 160 * 1024) {
+            constexpr size_t bytes = Chunks<T, NK>::kBytes;
+            if (a.segments > 1) {
+                if (const int rc = allow_lds<&delta_chunks_kernel<T, NK, WIDE, true>>(bytes)) return rc;
+                hipLaunchKernelGGL((delta_chunks_kernel<T, NK, WIDE, true>), dim3(heads * a.segments * (a.across / 64)), dim3(kThreads), bytes, st, a, slots, pl.groups);
+                RWKV_CHECK_LAUNCH("delta_chunks_kernel");
+                hipLaunchKernelGGL(delta_join_kernel<NK>, dim3(heads * ceil_div(a.dv, 16)), dim3(kThreads), 0, st, a, (int)ceil_div(a.dv, 16));
+                RWKV_CHECK_LAUNCH("delta_join_kernel");
+            }
+            if (const int rc = allow_lds<&delta_chunks_kernel<T, NK, WIDE, false>>(bytes)) return rc;
+            hipLaunchKernelGGL((delta_chunks_kernel<T, NK, WIDE, false>), dim3(heads * a.segments * pl.groups), dim3(kThreads), bytes, st, a, slots, pl.groups);
+            RWKV_CHECK_LAUNCH("delta_chunks_kernel");
+        } else {
+            constexpr size_t bytes = 2 * kChunk * (NK * 16 + 4) * 4;
+            if (const int rc = allow_lds<&delta_chunks_f32_kernel<T, NK, WIDE>>(bytes)) return rc;
+            hipLaunchKernelGGL((delta_chunks_f32_kernel<T, NK, WIDE>), dim3(heads * pl.groups), dim3(kThreads), bytes, st, a, slots, pl.groups);
+            RWKV_CHECK_LAUNCH("delta_chunks_f32_kernel");
+        }
         return (int)RWKV_OK;
     });
 }
@@ -733,8 +899,8 @@ using namespace rwkv;
 extern "C" {
 
 size_t rwkv_delta_rule_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv) {
-    if (T <= 0 || B <= 0 || Hv <= 0 || !in_chunks(T, B)) return 0;
-    return (size_t)((T / kChunk + B) * Hv) * kUnits * 16;
+    if (T <= 0 || B <= 0 || Hk <= 0 || Hv <= 0 || dk <= 0 || dv <= 0) return 0;
+    return DeltaPlan(T, B, Hv, dk, dv).bytes();
 }
 
 int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv, int type, const void *q,
@@ -746,23 +912,25 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
     RWKV_CHECK_ARG(starts || T % B == 0, "rwkv_delta_rule: rows must be a multiple of the sequences where there are no starts");
     RWKV_CHECK_ARG(type == RWKV_F32 || type == RWKV_BF16 || type == RWKV_F16, "rwkv_delta_rule: rows are float32, bfloat16 or float16");
     RWKV_CHECK_ARG(q_stride >= 0 && k_stride >= 0 && v_stride >= 0, "rwkv_delta_rule: negative row stride");
-    if (dk > 256 || dv > 65536 || Hv > 65535 || T >= (1ll << 31) || B * Hv * ceil_div(dv, 16) >= (1ll << 31))
+    if (dk > 256 || dv > 65536 || Hv > 65535 || T >= (1ll << 31) || B * Hv * ceil_div(dv, 16) >= (1ll << 27) || (T / 64 + B) * Hv >= (1ll << 30))
         return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: keys of at most 256 channels");
-    if (in_chunks(T, B)) {
+    const DeltaPlan pl(T, B, Hv, dk, dv);
+    if (pl.chunks) {
         if (q_stride >= (1 << 24) || k_stride >= (1 << 24) || v_stride >= (1 << 24) || Hv * dv >= (1 << 24))
             return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: rows of 2^24 elements or more");
         RWKV_CHECK_ALIGN(workspace, 16);
-        if (!workspace || workspace_bytes < rwkv_delta_rule_workspace_bytes(T, B, Hk, Hv, dk, dv))
+        if (!workspace || workspace_bytes < pl.bytes())
             return set_error(RWKV_ERR_WORKSPACE, "rwkv_delta_rule: workspace too small");
     }
-    const DeltaArgs a{T, B, T / B, (int)(Hv / Hk), (int)Hv, (int)dk, (int)dv, q, k, v, q_stride, k_stride, v_stride, g, beta, scale, starts, state, o};
+    const DeltaArgs a{T, B, T / B, (int)(Hv / Hk), (int)Hv, (int)dk, (int)dv, q, k, v, q_stride, k_stride, v_stride, g, beta, scale, starts, state, o,
+                      pl.segments, (float *)((uint8_t *)workspace + pl.slot_bytes), (float *)((uint8_t *)workspace + pl.slot_bytes + pl.end_bytes), 64 * pl.groups, pl.across};
     const size_t size = type_bytes(type);
     auto fits = [&](const void *at, int64_t stride, int64_t channels) { return ((uintptr_t)at | (uintptr_t)(stride * size) | (uintptr_t)(channels * size)) % 16 == 0; };
     // (heads of whole 16 bytes, which are also what a lane of delta_steps_kernel takes at a time, or multiples of it)
     const bool wide = fits(q, q_stride, dk) && fits(k, k_stride, dk) && fits(v, v_stride, dv) && (uintptr_t)state % 16 == 0 && (uintptr_t)o % 16 == 0 && dk % 16 == 0 && dv % 8 == 0;
     return with_low(type, [&](auto ty) {
         using E = typename decltype(ty)::type;
-        return wide ? launch<E, true>((hipStream_t)stream, a, (f32x4 *)workspace) : launch<E, false>((hipStream_t)stream, a, (f32x4 *)workspace);
+        return wide ? launch<E, true>((hipStream_t)stream, a, pl, (f32x4 *)workspace) : launch<E, false>((hipStream_t)stream, a, pl, (f32x4 *)workspace);
     });
 }
 

@@ -149,7 +149,16 @@ def test_delta_rule(ops, dtype, Hk, Hv, dk, dv, starts):
     _delta(ops, P.delta_inputs(starts[-1] + 5, len(starts) - 1, Hk, Hv, dk, dv, dtype, sum(starts) + dk), starts)
 
 
-@pytest.mark.parametrize("T,B", [(4, 4), (6, 2), (200, 2), (129, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hk,Hv,dk,dv,starts", [(1, 2, 64, 64, [0, 2500]), (1, 1, 33, 70, [0, 60, 2600]), (2, 4, 128, 128, [0, 1300]), (1, 1, 256, 24, [0, 1100]),
+                                                (1, 1, 20, 8, [5, 5, 70, 71, 5000]), (1, 3, 96, 200, [0, 1030, 2060])])
+def test_delta_rule_of_long_sequences(ops, dtype, Hk, Hv, dk, dv, starts):
+    """Few heads and long sequences: cut into segments, one sequence of a single segment among them."""
+    print(f"delta rule {Hk} {Hv} {dk} {dv} {starts} {dtype}", flush=True)
+    _delta(ops, P.delta_inputs(starts[-1] + 3, len(starts) - 1, Hk, Hv, dk, dv, dtype, sum(starts) + dk, rate=-6.0), starts)
+
+
+@pytest.mark.parametrize("T,B", [(4, 4), (6, 2), (200, 2), (129, 1), (1600, 2)])
 def test_delta_rule_without_starts(ops, T, B):
     c = P.delta_inputs(T, B, 2, 2, 64, 48, torch.float32, T)
     want, after = P.delta_rule(*c, [T // B * i for i in range(B + 1)], 0.25)
