@@ -254,19 +254,6 @@ template <typename V> __device__ __forceinline__ auto planes_of(V v) {
 }
 
 
-// 64 rows (zeros behind the n-th) of dk channels into LDS, as To, rows `stride` apart; WIDE: 16-byte aligned rows that fill whole 16 bytes.
-template <bool WIDE, typename To, typename T>
-__device__ __forceinline__ void stage(To *lds, int stride, int filled, const T *from, int64_t from_stride, int n, int dk) {
-    constexpr int E = WIDE ? 16 / sizeof(T) : 1;
-    const int per = filled / E;
-    for (int at = threadIdx.x; at < kChunk * per; at += blockDim.x) {
-        const int row = at / per, k = at % per * E;
-        const auto v = take<E, WIDE>(from + row * from_stride, k, row < n ? dk : 0);
-#pragma unroll
-        for (int e = 0; e < E; ++e) lds[row * stride + k + e] = (To)v[e];
-    }
-}
-
 // Products of 16 rows with 16 rows, lane (i, g) giving the i-th of each: the operands' own type where the matrix cores have it
 // (the products are exact), else float32.  The rows come from memory straight into the registers that the instruction reads.
 __device__ __forceinline__ f32x4 dot_step(Some<float, 4>::type l, Some<float, 4>::type r, f32x4 acc) { add_product(acc, l, r); return acc; }
@@ -400,6 +387,64 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
         if (m >= wave) slot[block_of(m, wave) * 64 + lane] = *reinterpret_cast<const f32x4 *>(&s_A[16 * m + i][16 * wave + 4 * g]);
 }
 
+// What a workgroup of the chunks goes through: a segment of a sequence, for 64 columns of a value head's state.
+// SUMMARY: a segment's N (the columns of the values, from 0 or, the first segment, from the state) and M (columns behind them, from the
+// identity, of no values); no outputs.
+struct Work {
+    int segment, h, hk, col0, col;
+    bool identity, at_end, in;
+    int64_t b, bh, begin, first, n;       // begin: chunks of the sequence in front of it; its rows
+    const f32x4 *slot;
+};
+template <bool SUMMARY> __device__ __forceinline__ bool work_of(const DeltaArgs &a, const f32x4 *slots, int groups, Work &w) {
+    const int places = SUMMARY ? a.across / 64 : groups, place = (int)(blockIdx.x % places);
+    const uint32_t unit = blockIdx.x / places, heads = (uint32_t)(a.B * a.Hv);          // (segments last: each compute unit gets some of all)
+    w.segment = (int)(unit / heads); w.h = (int)(unit % a.Hv); w.hk = w.h / a.share;
+    w.b = begun(a, unit % heads / a.Hv); w.bh = w.b * a.Hv + w.h;
+    w.identity = SUMMARY && place >= groups;
+    w.col0 = (place - (w.identity ? groups : 0)) * 64;
+    w.col = w.col0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 16 + (threadIdx.x & 15);
+    w.in = w.col < a.dv;
+    rows_of(a, w.b, w.first, w.n);
+    if (w.n <= 0) return false;
+    const int64_t chunks = segment_of(a, w.n, w.segment, w.begin);
+    w.at_end = (w.begin + chunks) * kChunk >= w.n;
+    if (chunks <= 0 || (SUMMARY && (w.at_end || (w.identity && w.segment == 0)))) return false;
+    w.slot = slots + ((place_of(w.first, w.b) + w.begin) * a.Hv + w.h) * kUnits;
+    w.first += w.begin * kChunk;
+    w.n = min(w.n - w.begin * kChunk, chunks * kChunk);
+    return true;
+}
+template <bool SUMMARY, int NK> __device__ __forceinline__ void begin_with(const DeltaArgs &a, const Work &w, f32x4 (&S)[NK]) {
+    float *const state = a.state + w.bh * a.dk * a.dv, *const front = a.fronts + (w.bh * a.segments + w.segment) * a.dk * a.dv;
+    const float *const from = SUMMARY || (w.segment == 0 && w.at_end) ? state : front;          // (a sequence of one segment has no summary)
+    const int g = threadIdx.x >> 4 & 3;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int row = 16 * k + 4 * g + v;
+            if (SUMMARY && (w.identity || w.segment)) S[k][v] = w.identity && row == w.col && row < a.dk ? 1.f : 0.f;
+            else {
+                S[k][v] = row < a.dk ? from[(int64_t)row * a.dv + (w.in ? w.col : 0)] : 0.f;
+                if (SUMMARY && w.in && row < a.dk) front[(int64_t)row * a.dv + w.col] = S[k][v];          // (the last segment writes the state while the first reads it)
+            }
+        }
+}
+template <bool SUMMARY, int NK> __device__ __forceinline__ void end_with(const DeltaArgs &a, const Work &w, int groups, const f32x4 (&S)[NK]) {
+    float *const state = a.state + w.bh * a.dk * a.dv, *const ends = a.ends + (w.bh * a.segments + w.segment) * a.dk * a.across + (w.identity ? groups * 64 : 0);
+    const int g = threadIdx.x >> 4 & 3;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int row = 16 * k + 4 * g + v;
+            if (row >= a.dk) continue;
+            if (SUMMARY) { if (!w.identity || w.col < NK * 16) ends[(int64_t)row * a.across + w.col] = S[k][v]; }
+            else if (w.at_end && w.in) state[(int64_t)row * a.dv + w.col] = S[k][v];
+        }
+}
+
 // NK tiles of 16 key channels; four wavefronts of 16 columns of the state each.  S, and what is multiplied with it and comes of it,
 // stay in the wavefront's registers; the left operands lie in LDS, where a lane's eight terms are 16 bytes:
 //   K, Q   [plane][row][block of 32 channels][unit g ^ (row / 16)], unit g: channels 4 g .. + 3 and 16 + 4 g .. + 3 of the block
@@ -415,8 +460,6 @@ template <typename T, int NK> struct Chunks {
     static constexpr int kRows = NK >= 8 ? 4 : 2, kPieces = NK * 2 * (kChunk / kRows) / kThreads;          // rows of a piece of K or Q, pieces of a thread
 };
 
-// SUMMARY: a segment's N (groups of columns of values, from 0 or, the first segment, from the state) and M (groups behind them, from
-// the identity, of no values); no outputs.
 template <typename T, int NK, bool WIDE, bool SUMMARY>
 __global__ void __launch_bounds__(kThreads, NK <= 4 ? 2 : 1) delta_chunks_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
     using C = Chunks<T, NK>;
@@ -425,22 +468,12 @@ __global__ void __launch_bounds__(kThreads, NK <= 4 ? 2 : 1) delta_chunks_kernel
     constexpr int kIn = C::kIn, kRows = C::kRows, kPieces = C::kPieces, kAcross = kChunk / kRows;
     extern __shared__ __align__(16) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
-    const int places = SUMMARY ? a.across / 64 : groups;
-    const uint32_t unit = blockIdx.x / places, heads = (uint32_t)(a.B * a.Hv);          // (segments last: each compute unit gets some of all)
-    const int segment = (int)(unit / heads), place = (int)(blockIdx.x % places), h = (int)(unit % a.Hv), hk = h / a.share;
-    const int64_t b = begun(a, unit % heads / a.Hv), bh = b * a.Hv + h;
-    const bool identity = SUMMARY && place >= groups;
-    const int col0 = (place - (identity ? groups : 0)) * 64, col = col0 + wave * 16 + i;
-    const bool in = col < a.dv;
-    int64_t first, n, begin;
-    rows_of(a, b, first, n);
-    if (n <= 0) return;
-    const int64_t chunks = segment_of(a, n, segment, begin);
-    const bool at_end = (begin + chunks) * kChunk >= n;
-    if (chunks <= 0 || (SUMMARY && (at_end || (identity && segment == 0)))) return;
-    const f32x4 *slot = slots + ((place_of(first, b) + begin) * a.Hv + h) * kUnits;
-    first += begin * kChunk;
-    n = min(n - begin * kChunk, chunks * kChunk);
+    Work w;
+    if (!work_of<SUMMARY>(a, slots, groups, w)) return;
+    const int h = w.h, hk = w.hk, col0 = w.col0;
+    const bool identity = w.identity;
+    const int64_t first = w.first, n = w.n;
+    const f32x4 *slot = w.slot;
     const int64_t end = (n - 1) / kChunk * kChunk;       // the last chunk
     // Offsets within a chunk fit 32 bits (the host has looked).  Rows behind the last are the last again, columns the first: T's
     // columns are 0 there, and what comes of them is not written.  Behind the last chunk it is fetched again.
@@ -556,20 +589,8 @@ __global__ void __launch_bounds__(kThreads, NK <= 4 ? 2 : 1) delta_chunks_kernel
     fetch_rows(0);
     fetch_rest(0);
     for (int at = tid; at < 2 * kPairs * 3 * 64; at += kThreads) reinterpret_cast<u32x4 *>(lds + C::kPairsAt)[at] = u32x4{0, 0, 0, 0};      // (pairs' blocks above the diagonal)
-    float *const state = a.state + bh * a.dk * a.dv, *const front = a.fronts + (bh * a.segments + segment) * a.dk * a.dv;
-    const float *const from_state = SUMMARY || (segment == 0 && at_end) ? state : front;          // (a sequence of one segment has no summary)
     f32x4 S[NK];
-#pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int row = 16 * k + 4 * g + v;
-            if (SUMMARY && (identity || segment)) S[k][v] = identity && row == col && row < a.dk ? 1.f : 0.f;
-            else {
-                S[k][v] = row < a.dk ? from_state[(int64_t)row * a.dv + (in ? col : 0)] : 0.f;
-                if (SUMMARY && in && row < a.dk) front[(int64_t)row * a.dv + col] = S[k][v];          // (the last segment writes the state while the first reads it)
-            }
-        }
+    begin_with<SUMMARY>(a, w, S);
     __syncthreads();
     auto keep = [&] {
 #pragma unroll
@@ -658,16 +679,7 @@ __global__ void __launch_bounds__(kThreads, NK <= 4 ? 2 : 1) delta_chunks_kernel
         }
         __syncthreads();
     }
-    float *const ends = a.ends + (bh * a.segments + segment) * a.dk * a.across + (identity ? groups * 64 : 0);
-#pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const int row = 16 * k + 4 * g + v;
-            if (row >= a.dk) continue;
-            if (SUMMARY) { if (identity ? col < NK * 16 : true) ends[(int64_t)row * a.across + col] = S[k][v]; }
-            else if (at_end && in) state[(int64_t)row * a.dv + col] = S[k][v];
-        }
+    end_with<SUMMARY>(a, w, groups, S);
 }
 
 // The state in front of each segment but the first: X_1 = N_0, X_(s+1) = N_s + M_s X_s, with float32 instructions.  A workgroup to 16
@@ -736,46 +748,69 @@ __global__ void __launch_bounds__(kThreads) delta_join_kernel(DeltaArgs a, int c
     }
 }
 
-// The same with float32 operands and instructions, where K, Q and K^T in planes are more than LDS holds.
-template <typename T, int NK, bool WIDE>
-__global__ void __launch_bounds__(256) delta_chunks_f32_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
-    constexpr int kRow = NK * 16 + 4;
+// The same with float32 operands and instructions, where K, Q and K^T in planes are more than LDS holds.  The instructions bound it
+// (some 6 of the 11 us of a chunk at 128 channels: 2048 rows, 32 heads of 128 x 128, float32, in three segments 92 + 10 + 138 us).
+template <typename T, int NK, bool WIDE, bool SUMMARY>
+__global__ void __launch_bounds__(kThreads) delta_chunks_f32_kernel(DeltaArgs a, const f32x4 *slots, int groups) {
+    constexpr int kRow = NK * 16 + 4, E = 16 / sizeof(T), kAcross = NK * 16 / E, kPieces = kChunk * kAcross / kThreads;          // (pieces of 16 bytes)
     extern __shared__ __align__(16) unsigned char smem[];
     float *ks = reinterpret_cast<float *>(smem), *qs = ks + kChunk * kRow;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-    const int h = (int)(blockIdx.x / groups % a.Hv), hk = h / a.share;
-    const int64_t b = blockIdx.x / groups / a.Hv;
-    const int col = (int)(blockIdx.x % groups) * (int)(blockDim.x >> 2) + wave * 16 + i;
-    const bool in = col < a.dv;
-    int64_t first, n;
-    rows_of(a, b, first, n);
-    if (n <= 0) return;
-    float *state = a.state + (b * a.Hv + h) * a.dk * a.dv + col;
+    Work w;
+    if (!work_of<SUMMARY>(a, slots, groups, w)) return;
+    const int h = w.h, hk = w.hk, col = w.col;
+    const bool in = w.in;
+    const int64_t first = w.first, n = w.n;
+    const f32x4 *slot = w.slot;
     f32x4 S[NK];
+    begin_with<SUMMARY>(a, w, S);
+    // Keys, queries and values of the next chunk are on the way during this one, T during the products with S, P as T is used.  (rows behind the
+    // last: the last again, as above)
+    typename Some<T, E>::type keys[kPieces], queries[kPieces];
+    T values[4][4];
+    auto fetch = [&](int64_t done) {
+        const int end = (int)min((int64_t)kChunk, n - done) - 1;
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
+        for (int m = 0; m < kPieces; ++m) {
+            const int at = m * kThreads + threadIdx.x;
+            const int64_t row = first + done + min(at / kAcross, end);
+            keys[m] = take<E, WIDE>((const T *)a.k + row * a.k_stride + (int64_t)hk * a.dk, at % kAcross * E, a.dk);
+            if (!SUMMARY) queries[m] = take<E, WIDE>((const T *)a.q + row * a.q_stride + (int64_t)hk * a.dk, at % kAcross * E, a.dk);
+        }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; S[k][v] = in && row < a.dk ? state[(int64_t)row * a.dv] : 0.f; }
-    const f32x4 *slot = slots + (place_of(first, b) * a.Hv + h) * kUnits;
-    for (int64_t done = 0; done < n; done += kChunk, first += kChunk, slot += (int64_t)a.Hv * kUnits) {
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) values[m][v] = w.identity ? (T)0.f : ((const T *)a.v)[(first + done + min(16 * m + 4 * g + v, end)) * a.v_stride + (int64_t)h * a.dv + (in ? col : 0)];
+    };
+    fetch(0);
+    const int64_t end = (n - 1) / kChunk * kChunk;
+    for (int64_t done = 0; done < n; done += kChunk, slot += (int64_t)a.Hv * kUnits) {
         const float *decays = reinterpret_cast<const float *>(slot + kUnitG);
         const int live = (int)min((int64_t)kChunk, n - done);
-        f32x4 R[4], eG[4], eL[4];
+        f32x4 R[4], eG[4], eL[4], blocks[kBlocks];
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < kPieces; ++m) {
+            const int at = m * kThreads + threadIdx.x;
+            float *to = ks + at / kAcross * kRow + at % kAcross * E, *other = qs + at / kAcross * kRow + at % kAcross * E;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                *reinterpret_cast<f32x4 *>(to + e) = f32x4{(float)keys[m][e], (float)keys[m][e + 1], (float)keys[m][e + 2], (float)keys[m][e + 3]};
+                if (!SUMMARY) *reinterpret_cast<f32x4 *>(other + e) = f32x4{(float)queries[m][e], (float)queries[m][e + 1], (float)queries[m][e + 2], (float)queries[m][e + 3]};
+            }
+        }
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int row = 16 * m + 4 * g + v;
-                R[m][v] = in && row < live ? (float)((const T *)a.v)[(first + row) * a.v_stride + (int64_t)h * a.dv + col] : 0.f;
-            }
+            for (int v = 0; v < 4; ++v) R[m][v] = (float)values[m][v];
             eG[m] = *reinterpret_cast<const f32x4 *>(decays + 16 * m + 4 * g);
             eL[m] = *reinterpret_cast<const f32x4 *>(decays + kChunk + 16 * m + 4 * g);
         }
+#pragma unroll
+        for (int at = 0; at < kBlocks; ++at) blocks[at] = slot[at * 64 + lane];
         const float last = decays[kChunk - 1];
         __syncthreads();
-        stage<WIDE>(ks, kRow, NK * 16, (const T *)a.k + first * a.k_stride + (int64_t)hk * a.dk, a.k_stride, live, a.dk);
-        stage<WIDE>(qs, kRow, NK * 16, (const T *)a.q + first * a.q_stride + (int64_t)hk * a.dk, a.q_stride, live, a.dk);
-        __syncthreads();
+        fetch(min(done + kChunk, end));
         f32x4 kS[4], O[4], U[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) { kS[m] = O[m] = U[m] = f32x4{0, 0, 0, 0}; }
@@ -784,24 +819,28 @@ __global__ void __launch_bounds__(256) delta_chunks_f32_kernel(DeltaArgs a, cons
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 add_product(kS[m], *reinterpret_cast<const f32x4 *>(ks + (16 * m + i) * kRow + 16 * k + 4 * g), S[k]);
-                add_product(O[m], *reinterpret_cast<const f32x4 *>(qs + (16 * m + i) * kRow + 16 * k + 4 * g), S[k]);
+                if (!SUMMARY) add_product(O[m], *reinterpret_cast<const f32x4 *>(qs + (16 * m + i) * kRow + 16 * k + 4 * g), S[k]);
             }
 #pragma unroll
         for (int m = 0; m < 4; ++m) { R[m] -= eG[m] * kS[m]; O[m] *= eG[m] * a.scale; }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int c = 0; c <= m; ++c) add_product(U[m], slot[block_of(m, c) * 64 + lane], R[c]);
+            for (int c = 0; c <= m; ++c) {
+                f32x4 &block = blocks[block_of(m, c)];
+                add_product(U[m], block, R[c]);
+                if (!SUMMARY) block = slot[kUnitP + block_of(m, c) * 64 + lane];
+            }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int c = 0; c <= m; ++c) add_product(O[m], slot[kUnitP + block_of(m, c) * 64 + lane], U[c]);
+            for (int c = 0; c <= m; ++c) if (!SUMMARY) add_product(O[m], blocks[block_of(m, c)], U[c]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const int row = 16 * m + 4 * g + v;
-                if (in && row < live) ((T *)a.o)[((first + row) * a.Hv + h) * a.dv + col] = (T)O[m][v];
+                if (!SUMMARY && in && row < live) ((T *)a.o)[((first + done + row) * a.Hv + h) * a.dv + col] = (T)O[m][v];
             }
             U[m] *= eL[m];
         }
@@ -815,10 +854,7 @@ __global__ void __launch_bounds__(256) delta_chunks_f32_kernel(DeltaArgs a, cons
                     S[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(ks[(16 * m + 4 * g + v) * kRow + 16 * k + i], U[m][v], S[k], 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) { const int row = 16 * k + 4 * g + v; if (in && row < a.dk) state[(int64_t)row * a.dv] = S[k][v]; }
+    end_with<SUMMARY>(a, w, groups, S);
 }
 
 // Chunks from this many rows a sequence on.
@@ -867,26 +903,27 @@ int launch(hipStream_t st, const DeltaArgs &a, const DeltaPlan &pl, f32x4 *slots
     RWKV_CHECK_LAUNCH("delta_within_kernel");
     return by_channels(a.dk, [&](auto nk) {
         constexpr int NK = decltype(nk)::value < 4 ? 4 : decltype(nk)::value;
-        const unsigned heads = (unsigned)(a.B * a.Hv);
-        if constexpr (Chunks<T, NK>::kBytes <= 160 * 1024) {
-            constexpr size_t bytes = Chunks<T, NK>::kBytes;
-            if (a.segments > 1) {
-                if (const int rc = allow_lds<&delta_chunks_kernel<T, NK, WIDE, true>>(bytes)) return rc;
-                hipLaunchKernelGGL((delta_chunks_kernel<T, NK, WIDE, true>), dim3(heads * a.segments * (a.across / 64)), dim3(kThreads), bytes, st, a, slots, pl.groups);
-                RWKV_CHECK_LAUNCH("delta_chunks_kernel");
-                hipLaunchKernelGGL(delta_join_kernel<NK>, dim3(heads * ceil_div(a.dv, 16)), dim3(kThreads), 0, st, a, (int)ceil_div(a.dv, 16));
-                RWKV_CHECK_LAUNCH("delta_join_kernel");
+        auto go = [&](auto summary) {
+            constexpr bool SUMMARY = decltype(summary)::value, PLANES = Chunks<T, NK>::kBytes <= 160 * 1024;
+            constexpr size_t bytes = PLANES ? Chunks<T, NK>::kBytes : 2 * kChunk * (NK * 16 + 4) * 4;
+            const dim3 grid((unsigned)(a.B * a.Hv * a.segments * (SUMMARY ? a.across / 64 : pl.groups)));
+            if constexpr (PLANES) {
+                if (const int rc = allow_lds<&delta_chunks_kernel<T, NK, WIDE, SUMMARY>>(bytes)) return rc;
+                hipLaunchKernelGGL((delta_chunks_kernel<T, NK, WIDE, SUMMARY>), grid, dim3(kThreads), bytes, st, a, slots, pl.groups);
+            } else {
+                if (const int rc = allow_lds<&delta_chunks_f32_kernel<T, NK, WIDE, SUMMARY>>(bytes)) return rc;
+                hipLaunchKernelGGL((delta_chunks_f32_kernel<T, NK, WIDE, SUMMARY>), grid, dim3(kThreads), bytes, st, a, slots, pl.groups);
             }
-            if (const int rc = allow_lds<&delta_chunks_kernel<T, NK, WIDE, false>>(bytes)) return rc;
-            hipLaunchKernelGGL((delta_chunks_kernel<T, NK, WIDE, false>), dim3(heads * a.segments * pl.groups), dim3(kThreads), bytes, st, a, slots, pl.groups);
             RWKV_CHECK_LAUNCH("delta_chunks_kernel");
-        } else {
-            constexpr size_t bytes = 2 * kChunk * (NK * 16 + 4) * 4;
-            if (const int rc = allow_lds<&delta_chunks_f32_kernel<T, NK, WIDE>>(bytes)) return rc;
-            hipLaunchKernelGGL((delta_chunks_f32_kernel<T, NK, WIDE>), dim3(heads * pl.groups), dim3(kThreads), bytes, st, a, slots, pl.groups);
-            RWKV_CHECK_LAUNCH("delta_chunks_f32_kernel");
+            return (int)RWKV_OK;
+        };
+        if (a.segments > 1) {
+            if (const int rc = go(std::true_type{})) return rc;
+            const int columns = (int)ceil_div(a.dv, 16);
+            hipLaunchKernelGGL(delta_join_kernel<NK>, dim3((unsigned)(a.B * a.Hv * columns)), dim3(kThreads), 0, st, a, columns);
+            RWKV_CHECK_LAUNCH("delta_join_kernel");
         }
-        return (int)RWKV_OK;
+        return go(std::false_type{});
     });
 }
 
