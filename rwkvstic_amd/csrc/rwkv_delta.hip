@@ -951,6 +951,12 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
     RWKV_CHECK_ARG(q_stride >= 0 && k_stride >= 0 && v_stride >= 0, "rwkv_delta_rule: negative row stride");
     if (dk > 256 || dv > 65536 || Hv > 65535 || T >= (1ll << 31) || B * Hv * ceil_div(dv, 16) >= (1ll << 27) || (T / 64 + B) * Hv >= (1ll << 30))
         return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: keys of at most 256 channels");
+    const int64_t e = (int64_t)type_bytes(type);
+    const int64_t o_bytes = T * Hv * dv * e, state_bytes = B * Hv * dk * dv * 4;
+    auto apart = [&](const void *from, int64_t bytes) { return !rows_share(1, o, 0, o_bytes, from, 0, bytes) && !rows_share(1, state, 0, state_bytes, from, 0, bytes); };
+    RWKV_CHECK_ARG(apart(q, ((T - 1) * q_stride + Hk * dk) * e) && apart(k, ((T - 1) * k_stride + Hk * dk) * e) && apart(v, ((T - 1) * v_stride + Hv * dv) * e) &&
+                       apart(g, T * Hv * 4) && apart(beta, T * Hv * 4) && !rows_share(1, o, 0, o_bytes, state, 0, state_bytes),
+                   "rwkv_delta_rule: o or state shares memory with another argument");
     const DeltaPlan pl(T, B, Hv, dk, dv);
     if (pl.chunks) {
         if (q_stride >= (1 << 24) || k_stride >= (1 << 24) || v_stride >= (1 << 24) || Hv * dv >= (1 << 24))

@@ -515,6 +515,10 @@ int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out,
     RWKV_CHECK_ARG(x_stride >= 0 && out_stride >= (T > 1 ? n_out : 0) && (!base || base_stride >= 0), "rwkv_lora_rows: row stride too small");
     if (R > 256 || T > (1 << 24) || n_in >= (1ll << 30) || n_out >= (1ll << 30) || N >= (1ll << 30))
         return set_error(RWKV_ERR_SIZE, "rwkv_lora_rows: too many rows, or a rank over 256");
+    if (base && (base != out || base_stride != out_stride)) {
+        const int64_t e = (int64_t)type_bytes(real);
+        RWKV_CHECK_ARG(!rows_share(T, base, base_stride * e, n_out * e, out, out_stride * e, n_out * e), "rwkv_lora_rows: out shares memory with base and is not base");
+    }
     RWKV_CHECK_ALIGN(workspace, 16);
     const LoraPlan pl(T, n_in, n_out, N, R, real);
     if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_lora_rows: workspace too small");

@@ -15,6 +15,16 @@ inline size_t type_bytes(int t) { return t == RWKV_F64 ? 8 : t == RWKV_F32 ? 4 :
 template <typename F> auto with_low(int t, F &&fn) { return t == RWKV_F32 ? fn(Elem<float>{}) : t == RWKV_BF16 ? fn(Elem<__bf16>{}) : fn(Elem<_Float16>{}); }
 template <typename F> auto with_real(int t, F &&fn) { return t == RWKV_F64 ? fn(Elem<double>{}) : fn(Elem<float>{}); }
 
+// Whether T rows of n bytes at a, and of m bytes at b, share memory; rows as many bytes apart as is said.  Rows equally far apart may lie
+// between each other.
+inline bool rows_share(int64_t T, const void *a, int64_t a_apart, int64_t n, const void *b, int64_t b_apart, int64_t m) {
+    const int64_t at = (int64_t)((uintptr_t)b - (uintptr_t)a);
+    if (at >= (T - 1) * a_apart + n || -at >= (T - 1) * b_apart + m) return false;
+    if (a_apart != b_apart || a_apart <= 0 || T == 1) return true;
+    const int64_t off = (at % a_apart + a_apart) % a_apart;
+    return off < n || off + m > a_apart;
+}
+
 // Lets a kernel have this much dynamic LDS where that is over the default limit; asked of the runtime once a device.
 template <auto Kernel> int allow_lds(size_t bytes) {
     if (bytes <= 65536) return RWKV_OK;

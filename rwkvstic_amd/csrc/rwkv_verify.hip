@@ -8,6 +8,8 @@
 // Of the logits the first kernel reads everything once; the others read one row of each a sequence (from cache).
 #include "rwkv_types.h"
 
+#include <algorithm>
+
 namespace rwkv {
 
 namespace {
@@ -439,7 +441,7 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
     uint8_t *ws = (uint8_t *)workspace;
     const bool of_drafts = draft_logits && !greedy && K > 0;
     const VerifyArgs a{B, K, V, logits, logits_seq_stride, logits_row_stride, of_drafts ? draft_logits : nullptr, draft_seq_stride, draft_row_stride,
-                       drafts, lengths, u, 1.0 / temp, tokens, accepted, pl.segments, pl.segment, (RowStat *)ws, pl.piece, (double *)(ws + pl.stat_bytes),
+                       drafts, lengths, u, 1.0 / std::max(temp, 1e-300), tokens, accepted, pl.segments, pl.segment, (RowStat *)ws, pl.piece, (double *)(ws + pl.stat_bytes),
                        (Verdict *)(ws + pl.stat_bytes + pl.sum_bytes)};
     const hipStream_t st = (hipStream_t)stream;
     const dim3 rows((unsigned)(B * (K + 1) + (of_drafts ? B * K : 0)), (unsigned)pl.segments), left((unsigned)B, (unsigned)pl.segments);

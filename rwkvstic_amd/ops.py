@@ -409,7 +409,8 @@ def lora_rows(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.
     ``x [T, n_in]`` and ``base [T, n_out]`` float32 or float64 (products and sums are computed in that type), ``a [N, R, n_in]``
     and ``b [N, n_out, R]`` bfloat16, float16 or float32 with ``R <= 256`` (adapters of smaller rank are filled up with zeros),
     ``adapter [T]`` int32: a row whose number is outside ``0..N-1`` has no adapter and gets ``base[t]``.  ``scale [N]`` float32;
-    without it 1.  ``base``: the shared projection's result, without it 0.  ``out`` may be ``base`` itself."""
+    without it 1.  ``base``: the shared projection's result, without it 0.  ``out`` may be ``base`` itself, and
+    shares no memory with it otherwise."""
     host = N.host()
     y = host and host.lora_rows(x, a, b, adapter, scale, base, out)
     if y is not None:
@@ -452,7 +453,8 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     value head ``h`` with key head ``h // (Hv // Hk)``; ``g`` (logarithm of the decay, at most 0) and ``beta [T, Hv]`` float32;
     ``state [B, Hv, dk, dv]`` float32, updated in place.  ``starts [B + 1]`` int32 on the device: sequence ``b`` is the rows
     ``starts[b]`` to ``starts[b + 1] - 1``; without it ``T / B`` rows each.  ``scale``: ``dk ** -0.5`` unless given.
-    Returns ``o [T, Hv, dv]`` of v's type; rows of no sequence are not written, and an empty sequence keeps its state."""
+    Returns ``o [T, Hv, dv]`` of v's type (``out``, which shares no memory with the arguments); rows of no sequence are not written,
+    and an empty sequence keeps its state."""
     scale = None if scale is None else float(scale)
     host = N.host()
     y = host and host.delta_rule(q, k, v, g, beta, state, starts, scale if scale is not None else _default_scale(q), out)

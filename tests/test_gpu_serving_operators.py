@@ -352,3 +352,16 @@ def test_tokens_follow_the_target_distribution(ops):
     want = torch.softmax(p, 0)
     count = torch.bincount(tokens[:, 0], minlength=V).double()
     assert bool(((count - n * want).abs() <= 6 * (n * want * (1 - want)).sqrt()).all())
+
+
+@pytest.mark.parametrize("temp", [1e-310, 5e-324])
+def test_hardly_any_temperature_is_none(ops, temp):
+    """All weight on the first maximum: a temperature whose reciprocal overflows gives the greedy choice."""
+    g = torch.Generator().manual_seed(5)
+    logits = torch.randn(4, 3, 700, generator=g, dtype=torch.float64)
+    drafts = logits[:, :2].argmax(-1)
+    drafts[1, 0] = (drafts[1, 0] + 1) % 700
+    u = torch.rand(4, 3, generator=g)
+    want = ops.verify_drafts(logits.cuda(), drafts.cuda(), greedy=True)
+    got = ops.verify_drafts(logits.cuda(), drafts.cuda(), u.cuda(), temp=temp)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)), (got, want)

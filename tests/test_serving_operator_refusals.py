@@ -98,3 +98,27 @@ def test_the_library_looks_for_itself():
         assert verify(**kw) == ARG, kw
     assert verify(K=65) == SIZE and verify(n=0) == WORKSPACE and verify(work=8) == ALIGN
     assert L.rwkv_verify_drafts_workspace_bytes(0, 3, 50) == 0
+
+
+def test_results_in_the_memory_of_what_is_read():
+    """Rows of base and of the result may lie between each other, and be the same; nothing is launched."""
+    from rwkvstic_amd import _native
+    L = _native.lib()
+    ARG, WORKSPACE, base = -1, -4, 1 << 20
+
+    def lora(T, at, bs, os, n_out=8):
+        return L.rwkv_lora_rows(None, T, 8, n_out, 1, 4, 0, 16, 8, 2, 16, 16, 16, None, base, bs, base + 4 * at, os, 16, 0)
+    for at, bs, os, shared in [(0, 8, 8, False), (0, 8, 9, True), (8, 8, 8, True), (24, 8, 8, False), (-24, 8, 8, False), (-23, 8, 8, True), (8, 16, 16, False),
+                               (-8, 16, 16, False), (7, 16, 16, True), (9, 16, 16, True), (9, 17, 17, False), (24, 8, 100, False), (5, 0, 8, True), (8, 0, 8, False)]:
+        assert lora(3, at, bs, os) == (ARG if shared else WORKSPACE), (at, bs, os)
+    assert lora(1, 8, 8, 8) == WORKSPACE and lora(1, 7, 8, 8) == ARG
+
+    far = [(i + 1) << 24 for i in range(7)]
+
+    def delta(**at):
+        q, k, v, g, beta, state, o = [at.get(n, f) for n, f in zip(("q", "k", "v", "g", "beta", "state", "o"), far)]
+        return L.rwkv_delta_rule(None, 100, 1, 1, 2, 16, 16, 0, q, 16, k, 16, v, 32, g, beta, 1.0, None, state, o, 16, 0)
+    assert delta() == WORKSPACE and delta(k=far[0]) == WORKSPACE
+    for kw in ({"o": far[2]}, {"o": far[0] + 4}, {"o": far[5]}, {"state": far[4]}, {"o": far[3] + 800 - 4}, {"o": far[1] - 4 * 3200 + 4}):
+        assert delta(**kw) == ARG, kw
+    assert delta(o=far[3] + 800) == WORKSPACE and delta(o=far[1] - 4 * 3200) == WORKSPACE
