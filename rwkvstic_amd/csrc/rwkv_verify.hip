@@ -5,7 +5,8 @@
 //   verify_rows_kernel  largest logit, and sum of the weights beside it (or first maximum), of every segment of every row
 //   verify_left_kernel  which drafts are accepted, and the sums of what the next token is drawn from, piece by piece
 //   verify_pick_kernel  the piece that the drawn token is in, and the token
-// Of the logits the first kernel reads everything once; the others read one row of each a sequence (from cache).
+// Of the logits the first kernel reads everything once; the others read one row of each a sequence (from cache).  64 sequences of
+// 8 drafts, 65536 tokens, float32, with the drafts' logits: 63 us (4.5 TB/s) + 20 + 7; one of 4, 50277 tokens, float64: 5 + 6 + 6, latency.
 #include "rwkv_types.h"
 
 #include <algorithm>
