@@ -263,13 +263,14 @@ __device__ __forceinline__ f32x4 dot_step(Some<__bf16, 8>::type l, Some<__bf16, 
 __device__ __forceinline__ f32x4 dot_step(Some<_Float16, 8>::type l, Some<_Float16, 8>::type r, f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(l, r, acc, 0, 0, 0); }
 
 // T and P of one chunk and value head; (1 + A)^-1 by blocks of 16.  A chain of short dependent parts bounds it (640 workgroups of 64
-// channels, float32: 23 us; 4096 of 128, bfloat16: 87 us).
+// channels, float32: 18.5 us; 4096 of 128, bfloat16: 68 us).  Blocks go to the wavefronts by rows: dealt out evenly they need twice the
+// loads (23 and 87 us).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *slots) {
     __shared__ double s_G[kChunk];
     __shared__ float s_beta[kChunk];
     __shared__ __align__(16) float s_A[kChunk][kChunk + 4], s_X[4][16][20];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, g = lane >> 4;
     const int h = blockIdx.y, hk = h / a.share;
     const int64_t place = blockIdx.x;
     // the last sequence whose places begin here or before
@@ -302,46 +303,49 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
         decays[lane] = expf((float)G);
         decays[kChunk + lane] = expf((float)(__shfl(G, 63, 64) - G));
     }
-    // transposed products, so that a lane has four neighbours of a row: of the wavefront's three blocks (or two) one row and its columns
-    constexpr int E = sizeof(T) == 4 ? 4 : 8, kMost = 3;
-    f32x4 kk[kMost], qk[kMost];
-    const T *kr[kMost], *qr[kMost], *kc[kMost];
+    // transposed products, so that a lane has four neighbours of a row: of the wavefront's row of blocks, whose keys are an operand of all
+    constexpr int E = sizeof(T) == 4 ? 4 : 8;
+    f32x4 kk[4], qk[4];
 #pragma unroll
-    for (int x = 0; x < kMost; ++x) {
-        kk[x] = qk[x] = f32x4{0, 0, 0, 0};
-        const int block = max(kBlocks - 1 - wave - 4 * x, 0), m = row_of(block);
-        const int row = min(16 * m + i, live - 1), column = min(16 * (block - block_of(m, 0)) + i, live - 1);
-        kr[x] = keys + row * a.k_stride; qr[x] = queries + row * a.q_stride; kc[x] = keys + column * a.k_stride;
-    }
-    auto terms = [&](int k, auto whole) {                 // (whole: none of the block's 4 E terms is behind the last)
-        auto some = [&](const T *row) {
-            if constexpr (decltype(whole)::value && WIDE) return *reinterpret_cast<const typename Some<T, E>::type *>(row + k);
-            else return take<E, WIDE>(row, k, a.dk);
+    for (int c = 0; c < 4; ++c) kk[c] = qk[c] = f32x4{0, 0, 0, 0};
+    auto products = [&](auto count) {
+        constexpr int N = decltype(count)::value;            // blocks of the row
+        const T *kr[N], *qr = queries + min(16 * (N - 1) + i, live - 1) * a.q_stride;
+#pragma unroll
+        for (int c = 0; c < N; ++c) kr[c] = keys + min(16 * c + i, live - 1) * a.k_stride;
+        auto terms = [&](int k, auto whole) {                 // (whole: none of the block's 4 E terms is behind the last)
+            auto some = [&](const T *row) {
+                if constexpr (decltype(whole)::value && WIDE) return *reinterpret_cast<const typename Some<T, E>::type *>(row + k);
+                else return take<E, WIDE>(row, k, a.dk);
+            };
+            typename Some<T, E>::type l[N], q = some(qr);
+#pragma unroll
+            for (int c = 0; c < N; ++c) l[c] = some(kr[c]);
+#pragma unroll
+            for (int c = 0; c < N; ++c) { kk[c] = dot_step(l[c], l[N - 1], kk[c]); qk[c] = dot_step(l[c], q, qk[c]); }
         };
-        typename Some<T, E>::type l[kMost], r[kMost], q[kMost];
-#pragma unroll
-        for (int x = 0; x < kMost; ++x) { l[x] = some(kc[x]); r[x] = some(kr[x]); q[x] = some(qr[x]); }
-#pragma unroll
-        for (int x = 0; x < kMost; ++x) { kk[x] = dot_step(l[x], r[x], kk[x]); qk[x] = dot_step(l[x], q[x], qk[x]); }
+        int k = 0;
+#pragma unroll 4
+        for (; k + 4 * E <= a.dk; k += 4 * E) terms(k + E * g, std::true_type{});
+        if (k < a.dk) terms(k + E * g, std::false_type{});
     };
-    int k = 0;
-#pragma unroll 2
-    for (; k + 4 * E <= a.dk; k += 4 * E) terms(k + E * g, std::true_type{});
-    if (k < a.dk) terms(k + E * g, std::false_type{});
+    if (wave == 0) products(std::integral_constant<int, 1>{});
+    else if (wave == 1) products(std::integral_constant<int, 2>{});
+    else if (wave == 2) products(std::integral_constant<int, 3>{});
+    else products(std::integral_constant<int, 4>{});
     __syncthreads();
     // A into LDS, P out
 #pragma unroll
-    for (int x = 0; x < kMost; ++x) {
-        const int block = kBlocks - 1 - wave - 4 * x;
-        if (block < 0) continue;
-        const int m = row_of(block), c = block - block_of(m, 0), row = 16 * m + i;
+    for (int c = 0; c < 4; ++c) {
+        if (c > wave) break;
+        const int block = block_of(wave, c), row = 16 * wave + i;
         f32x4 A, P;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const int column = 16 * c + 4 * g + v;
             const float decay = expf((float)(s_G[row] - s_G[column]));
-            A[v] = column < row ? s_beta[row] * decay * kk[x][v] : 0.f;
-            P[v] = column <= row ? a.scale * decay * qk[x][v] : 0.f;
+            A[v] = column < row ? s_beta[row] * decay * kk[c][v] : 0.f;
+            P[v] = column <= row ? a.scale * decay * qk[c][v] : 0.f;
         }
         *reinterpret_cast<f32x4 *>(&s_A[row][16 * c + 4 * g]) = A;
         slot[kUnitP + block * 64 + lane] = P;
@@ -361,21 +365,16 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
         for (int r = 0; r < 16; ++r) s_X[wave][r][lane] = x[r];
     }
     __syncthreads();
-    // ... the others below them, a wavefront to a column of blocks: X_mc = -X_mm sum_l A_ml X_lc
+    // ... the others below them, a wavefront to a column of blocks: X_mc = -X_mm sum_l A_ml X_lc; 0 above the diagonal, without branches
     f32x4 X[4];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-        X[m] = f32x4{0, 0, 0, 0};
-        if (m == wave) {
+        f32x4 Y = {0, 0, 0, 0}, below = {0, 0, 0, 0};
 #pragma unroll
-            for (int v = 0; v < 4; ++v) X[m][v] = s_X[m][4 * g + v][i];
-        } else if (m > wave) {
-            f32x4 Y = {0, 0, 0, 0};
+        for (int l = 0; l < m; ++l) add_product(Y, *reinterpret_cast<const f32x4 *>(&s_A[16 * m + i][16 * l + 4 * g]), X[l]);
+        if (m) add_product(below, *reinterpret_cast<const f32x4 *>(&s_X[m][i][4 * g]), -Y);
 #pragma unroll
-            for (int l = 0; l < m; ++l)
-                if (l >= wave) add_product(Y, *reinterpret_cast<const f32x4 *>(&s_A[16 * m + i][16 * l + 4 * g]), X[l]);
-            add_product(X[m], *reinterpret_cast<const f32x4 *>(&s_X[m][i][4 * g]), -Y);
-        }
+        for (int v = 0; v < 4; ++v) X[m][v] = m == wave ? s_X[m][4 * g + v][i] : m > wave ? below[v] : 0.f;
     }
     __syncthreads();
     // by rows again, through LDS: a wavefront writes and reads its own columns only

@@ -365,3 +365,22 @@ def test_hardly_any_temperature_is_none(ops, temp):
     want = ops.verify_drafts(logits.cuda(), drafts.cuda(), greedy=True)
     got = ops.verify_drafts(logits.cuda(), drafts.cuda(), u.cuda(), temp=temp)
     assert all(torch.equal(a, b) for a, b in zip(got, want)), (got, want)
+
+
+@pytest.mark.parametrize("T", [63, 64, 65, 127, 128, 129])
+def test_adapters_where_tiles_are_found_another_way(ops, T):
+    c = _adapters(T, 70, 50, 3, 5, torch.float32, torch.float16, T)
+    c["adapter"][::7] = -1
+    want, bound = P.lora_rows(**c)
+    _near(ops.lora_rows(**{k: v.cuda() for k, v in c.items()}), want, bound, HALF[torch.float32])
+
+
+@pytest.mark.parametrize("B", [64, 65])
+def test_delta_rule_of_many_ragged_sequences_in_chunks(ops, B):
+    """The longest begun first, up to a wavefront's number of sequences: equal ones, empty ones, the longest last."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 60, (B,), generator=g)
+    lens[:5], lens[9], lens[-1] = 0, 0, 60 * B
+    starts = [0] + lens.cumsum(0).tolist()
+    assert starts[-1] >= 64 * B
+    _delta(ops, P.delta_inputs(starts[-1], B, 1, 2, 16, 24, torch.float32, B, rate=-3.0), starts)
