@@ -365,7 +365,8 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
         for (int r = 0; r < 16; ++r) s_X[wave][r][lane] = x[r];
     }
     __syncthreads();
-    // ... the others below them, a wavefront to a column of blocks: X_mc = -X_mm sum_l A_ml X_lc; 0 above the diagonal, without branches
+    // ... the others below them, a wavefront to a column of blocks: X_mc = -X_mm sum_l A_ml X_lc; 0 above the diagonal.  Without
+    // branches: behind one on the wavefront's number the compiler left out the wait (10 instructions) that reading a product's registers needs.
     f32x4 X[4];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
