@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(64 * kDownWaves) lora_down_kernel(LoraArgs p) 
     const int row0 = place % parts * NT * 16, rank0 = blockIdx.z * RT * 16;
     Tile tile;
     if (!find_tile(p, place / parts, tile, rows) || tile.adapter < 0 || row0 >= tile.n) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    // (wave the same for all lanes: the loop's bounds are scalar then, and its matrix instructions, which do not look at EXEC, stand behind no mask)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const Real *x[NT];
 #pragma unroll
     for (int s = 0; s < NT; ++s) x[s] = (const Real *)p.x + (int64_t)rows[min(row0 + s * 16 + i, tile.n - 1)] * p.x_stride;
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
         return;
     }
     if (NT == 1 && sizeof(Real) == 8 && !p.order && tile.n <= kFew) { up_few<Real, Low, WIDE>(p, tile, rows, reinterpret_cast<Real *>(hs), n0, n1); return; }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const Low *b = (const Low *)p.b + (int64_t)tile.adapter * p.n_out * p.R;
     // QT tiles of outputs: lane (j, g) comes out with n + 16 q + 4 g .. + 3 of row j, 64 bytes of a row (128 of float64) to a store
     struct Rows { Eight<Low> v[QT][RB]; };
