@@ -72,11 +72,24 @@ __device__ __forceinline__ void load8(Eight<T> &to, const T *row, int64_t k, int
     }
 }
 
+template <typename Real, typename Low>
+__device__ __forceinline__ void add_whole(typename Four<Real>::type &acc, const Eight<Low> &l, const Eight<Real> &r) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = mfma((Real)l.e[e], r.e[e], acc);
+}
+// Whether one of four values is no number, and those of them that are none from another four.
+__device__ __forceinline__ bool no_number(f32x4 v) { return __builtin_isunordered(v[0], v[1]) || __builtin_isunordered(v[2], v[3]); }
+__device__ __forceinline__ void numbers(f32x4 &v, f32x4 others) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = v[c] == v[c] ? v[c] : others[c];
+}
+
 // What the matrix instructions make of eight terms (32 with the other lanes'): left operand from an adapter, right one from x or h.
 // In LDS the right operands of a row of n lie in planes [rows][n + pad]; the pad leaves rows an odd number of 16 bytes apart.
 template <typename Real, typename Low> struct Product {
     using Vec = typename Four<Real>::type;
     using Right = Eight<Real>;
+    static constexpr bool kParts = false;
     static constexpr int kPad = 16 / sizeof(Real);
     static constexpr int row_bytes(int n) { return (n + kPad) * sizeof(Real); }
     static __device__ __forceinline__ Right right(const Eight<Real> &v) { return v; }
@@ -88,18 +101,18 @@ template <typename Real, typename Low> struct Product {
         load8<true>(r, reinterpret_cast<const Real *>(lds) + row * (n + kPad), k, n);
         return r;
     }
-    static __device__ __forceinline__ void add(Vec &acc, const Eight<Low> &l, const Right &r) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc = mfma((Real)l.e[e], r.e[e], acc);
-    }
+    static __device__ __forceinline__ void add(Vec &acc, const Eight<Low> &l, const Right &r) { add_whole(acc, l, r); }
 };
 
 // float32 rows and bfloat16 adapters: a float32 value is the sum of three bfloat16 ones, its 24 bits cut in three, so that three
-// bfloat16 products with float32 sums lose nothing, in a fifth of the matrix cores' time for float32 operands.
+// bfloat16 products with float32 sums lose nothing, in a fifth of the matrix cores' time for float32 operands.  But for infinities:
+// one has no rest, and a part that is 0 must not meet one.  A sum with an infinite term comes out as no number, or right; the sums that
+// are none are taken again of whole operands (kParts), so that they are what the other types' are.
 template <> struct Product<float, __bf16> {
     typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
     using Vec = f32x4;
     struct Right { u32x4 part[3]; };
+    static constexpr bool kParts = true;
     static constexpr int kPad = 8;
     static constexpr int row_bytes(int n) { return 3 * (n + kPad) * 2; }
     static __device__ __forceinline__ float rest(float v) { return v - __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
@@ -119,8 +132,14 @@ template <> struct Product<float, __bf16> {
         for (int part = 0; part < 3; ++part) {
             *reinterpret_cast<uint2 *>(lds + ((part * rows + row) * (n + kPad) + k) * 2) = make_uint2(upper(f[0], f[1]), upper(f[2], f[3]));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = rest(f[i]);
+            for (int i = 0; i < 4; ++i) f[i] = fabsf(f[i]) == INFINITY ? 0.f : rest(f[i]);          // (so that the parts add up to the value)
         }
+    }
+    static __device__ __forceinline__ float whole(const unsigned char *lds, int rows, int n, int row, int k) {
+        float v = 0.f;
+#pragma unroll
+        for (int part = 2; part >= 0; --part) v += (float)*reinterpret_cast<const __bf16 *>(lds + ((part * rows + row) * (n + kPad) + k) * 2);
+        return v;
     }
     static __device__ __forceinline__ Right get(const unsigned char *lds, int rows, int n, int row, int k) {
         Right r;
@@ -270,6 +289,22 @@ __global__ void __launch_bounds__(64 * kDownWaves) lora_down_kernel(LoraArgs p) 
         load(even, k + 64);
         if (k + 32 < k1) multiply(odd);
     }
+    if constexpr (Op::kParts) {
+        bool again = false;
+#pragma unroll
+        for (int c = 0; c < NT * RT; ++c) again |= no_number(acc[c / RT][c % RT]);
+        if (__any(again)) {
+            Vec whole[NT][RT] = {};
+#pragma unroll 1
+            for (int64_t k = k0; k < k1; k += 32) {
+                load(even, k);
+#pragma unroll
+                for (int c = 0; c < NT * RT; ++c) add_whole(whole[c / RT][c % RT], even.a[c % RT], even.x[c / RT]);
+            }
+#pragma unroll
+            for (int c = 0; c < NT * RT; ++c) numbers(acc[c / RT][c % RT], whole[c / RT][c % RT]);
+        }
+    }
 #pragma unroll
     for (int half = kDownWaves / 2; half >= 1; half /= 2) {
         if (half < kDownWaves / 2) __syncthreads();
@@ -332,9 +367,10 @@ __device__ __forceinline__ void up_few(const LoraArgs &p, const Tile &tile, cons
 }
 
 // RB blocks of 32 ranks, NT times 16 rows of the tile: as many as 64 KiB of LDS hold.  An XCD takes the same ranges of outputs
-// for all tiles, and so reads these rows of b once.
+// for all tiles, and so reads these rows of b once.  Two wavefronts to a SIMD for operands in parts: where sums are taken
+// again the compiler would use the registers of one (2048 rows of 5120 to 5120, rank 256: 74 us, and 109 with one).
 template <typename Real, typename Low, int RB, int NT, int QT, bool WIDE>
-__global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
+__global__ void __launch_bounds__(256, (Product<Real, Low>::kParts && WIDE && NT > 1 ? 2 : 1)) lora_up_kernel(LoraArgs p) {
     using Op = Product<Real, Low>;
     using Vec = typename Op::Vec;
     extern __shared__ __align__(16) unsigned char hs[];                        // right operands of the tile's rows
@@ -363,10 +399,11 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
     const Low *b = (const Low *)p.b + (int64_t)tile.adapter * p.n_out * p.R;
     // QT tiles of outputs: lane (j, g) comes out with n + 16 q + 4 g .. + 3 of row j, 64 bytes of a row (128 of float64) to a store
     struct Rows { Eight<Low> v[QT][RB]; };
+    auto row_of = [&](int64_t n, int q) { return b + min(n + 16 * q + left_row<Real>(i), p.n_out - 1) * p.R; };
     auto load = [&](Rows &to, int64_t n) {
 #pragma unroll
         for (int q = 0; q < QT; ++q) {
-            const Low *row = b + min(n + 16 * q + left_row<Real>(i), p.n_out - 1) * p.R;
+            const Low *row = row_of(n, q);
 #pragma unroll
             for (int k = 0; k < RB; ++k) load8<WIDE>(to.v[q][k], row, k * 32 + 8 * g, p.R);
         }
@@ -424,6 +461,23 @@ __global__ void __launch_bounds__(256) lora_up_kernel(LoraArgs p) {
                 const typename Op::Right r = Op::get(hs, NT * 16, RB * 32, s * 16 + i, k * 32 + 8 * g);
 #pragma unroll
                 for (int q = 0; q < QT; ++q) Op::add(acc[q], now.v[q][k], r);
+            }
+            if constexpr (Op::kParts) {
+                bool again = false;
+#pragma unroll
+                for (int q = 0; q < QT; ++q) again |= no_number(acc[q]);
+                if (__any(again && s * 16 + i < n_rows)) {
+#pragma unroll
+                    for (int q = 0; q < QT; ++q) {
+                        Vec whole = {0, 0, 0, 0};
+#pragma unroll 1
+                        for (int term = 0; term < RB * 8; ++term) {          // (one at a time, for what that takes of registers)
+                            const int k = term / 8 * 32 + 8 * g + term % 8;
+                            whole = mfma(k < p.R ? (float)row_of(n, q)[k] : 0.f, Op::whole(hs, NT * 16, RB * 32, s * 16 + i, k), whole);
+                        }
+                        numbers(acc[q], whole);
+                    }
+                }
             }
             if (s * 16 + i >= n_rows) continue;
             Real *to = out + (int64_t)rows[row0 + s * 16 + i] * p.out_stride + n + 4 * g;
