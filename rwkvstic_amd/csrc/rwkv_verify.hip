@@ -47,18 +47,20 @@ struct VerifyArgs {
     Verdict *verdict;                // [B]
 };
 
-// e^(d / temp) for d <= 0 (0 for anything that is not a number), to 2^-47 or so: the exponent in 32nds of log2 e from a table, the
-// rest by its series (P. T. P. Tang, ACM TOMS 15, 1989).  Half the instructions of exp(), which takes longer than the logits
-// take to come; 2^-47 moves one draw in 10^9.
+// e^(d / temp) for d <= 0 (0 for anything that is not a number), to 2^-51 or so of it: the exponent in 32nds of log2 e from a table, the
+// rest by its series (P. T. P. Tang, ACM TOMS 15, 1989) to the sixth power (the seventh is below 2^-57).  Half the instructions of exp(),
+// which takes longer than the logits take to come.
 struct Exp {
     const double *table;                             // LDS: 2^(i/32)
-    double scale;                                    // 32 log2 e / temp
+    double inv_temp;
     __device__ __forceinline__ double operator()(double d) const {
         constexpr double kMagic = 6755399441055744.0;                        // 3 * 2^51: adding it rounds to a whole number
-        const double y = fmax(d * scale, -37000.0);                          // (2^(-37000 / 32) is 0; what is no number gives way to it)
-        const double z = y + kMagic, f = y - (z - kMagic);
+        constexpr double k32 = 46.16624130844683;                            // 32 log2 e, to 2^-56 of it
+        const double y = fmax(d * inv_temp, -800.0);                         // (2^-1154 is 0; what is no number gives way to it)
+        const double z = fma(y, k32, kMagic), f = fma(y, k32, -(z - kMagic));
         const int n = (int)__double_as_longlong(z);
-        double p = fma(f, 3.9737099845494161e-11, 9.1725627018246432e-09);          // (ln 2 / 32)^k / k!
+        double p = fma(f, 1.4345655584131934e-13, 3.9737099845494161e-11);          // (ln 2 / 32)^k / k!
+        p = fma(f, p, 9.1725627018246432e-09);
         p = fma(f, p, 1.6938509724371820e-06);
         p = fma(f, p, 2.3459619820224679e-04);
         p = fma(f, p, 2.1660849392498291e-02);
@@ -77,7 +79,7 @@ __constant__ const double kTable[32] = {               // 2^(i/32)
     1.8340080864093424635, 1.8741676341102999013, 1.9152065613971472939, 1.9571441241754002690};
 __device__ __forceinline__ Exp exp_table(double (&table)[32], double inv_temp) {              // (before a barrier)
     if (threadIdx.x < 32) table[threadIdx.x] = kTable[threadIdx.x];
-    return {table, inv_temp * 46.166241308446829};
+    return {table, inv_temp};
 }
 
 // A logit's weight beside the largest; NaN and -infinity have none, and where the largest is +infinity the others have none.
