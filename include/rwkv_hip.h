@@ -444,7 +444,8 @@ typedef enum rwkv_type { RWKV_F32 = 0, RWKV_F64 = 1, RWKV_BF16 = 2, RWKV_F16 = 3
  * RWKV_F16 or RWKV_F32), R <= 256 (adapters of smaller rank are filled with
  * zeros); adapter int32 [T]: a row whose number is not in 0..N-1 has none and
  * gets base[t].  scale float32 [N] or NULL (= 1); base NULL (= 0) or any rows: out
- * itself, or rows that share no memory with it.  What a row holds (infinities, NaN) reaches no other row.
+ * itself, or rows that share no memory with it.  out may lie over x, not over a, b, adapter or scale.
+ * What a row holds (infinities, NaN) reaches no other row.
  * workspace: rwkv_lora_rows_workspace_bytes bytes, 16-byte aligned. */
 size_t rwkv_lora_rows_workspace_bytes(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real);
 int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R,

@@ -500,7 +500,7 @@ struct LoraPlan {
     int windows, slots;                   // tiles are looked for in windows * slots places
     int group, groups, ranks;             // tiles of 16 ranks to a wavefront of lora_down_kernel, and wavefronts; ranks: 32, 64, 128 or 256
     int slices, steps, range, chunks;
-    size_t h_bytes, order_bytes, tile_bytes;
+    size_t h_bytes, order, tile_bytes;
     LoraPlan(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real) {
         direct = T <= kDirect;
         windows = direct ? 1 : (int)ceil_div(T, kWindow);
@@ -522,10 +522,10 @@ struct LoraPlan {
         chunks = (int)ceil_div(n_out, range);
         if (chunks > 8) chunks = (int)round_up(chunks, 8);
         h_bytes = round_up((size_t)slices * T * ranks * type_bytes(real), 256);
-        order_bytes = direct ? 0 : round_up((size_t)T * 4, 256);
+        order = direct ? 0 : round_up((size_t)T * 4, 256);
         tile_bytes = direct ? 0 : (size_t)windows * slots * sizeof(Tile);
     }
-    size_t bytes() const { return h_bytes + order_bytes + tile_bytes; }
+    size_t bytes() const { return h_bytes + order + tile_bytes; }
 };
 
 template <typename Real, typename Low, bool WIDE>
@@ -585,10 +585,14 @@ int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out,
     RWKV_CHECK_ALIGN(workspace, 16);
     const LoraPlan pl(T, n_in, n_out, N, R, real);
     if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_lora_rows: workspace too small");
+    // (x aside: it has been read when the first output is written)
+    const int64_t er = (int64_t)type_bytes(real), el = (int64_t)type_bytes(low);
+    auto apart = [&](const void *from, int64_t bytes) { return !from || !rows_share(T, out, out_stride * er, n_out * er, from, 0, bytes); };
+    RWKV_CHECK_ARG(apart(a, N * R * n_in * el) && apart(b, N * n_out * R * el) && apart(adapter, T * 4) && apart(scale, N * 4),
+                   "rwkv_lora_rows: out shares memory with an argument");
     uint8_t *ws = (uint8_t *)workspace;
     const LoraArgs p{T, n_in, n_out, N, R, x, x_stride, a, b, adapter, scale, base, base_stride, out, out_stride, pl.slices, pl.steps, pl.range, pl.chunks, pl.ranks,
-                     ws, pl.direct ? nullptr : (int32_t *)(ws + pl.h_bytes), (Tile *)(ws + pl.h_bytes + pl.order_bytes)};
-    const size_t er = type_bytes(real), el = type_bytes(low);
+                     ws, pl.direct ? nullptr : (int32_t *)(ws + pl.h_bytes), (Tile *)(ws + pl.h_bytes + pl.order)};
     auto fits = [](const void *at, int64_t elements, size_t size) { return ((uintptr_t)at | (uintptr_t)(elements * size)) % 16 == 0; };
     // (a row of four outputs may be 32 bytes, which 16-byte alignment serves)
     const bool wide = fits(x, x_stride, er) && fits(a, n_in, el) && fits(x, n_in, er) && fits(b, R, el) && fits(out, out_stride, er) && n_out % 4 == 0 &&

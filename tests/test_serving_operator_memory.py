@@ -1,0 +1,51 @@
+"""Results in the memory of what is read: refused by the library before anything is launched, and served where they only lie beside it."""
+import pytest
+import torch
+
+import serving_plain as P
+
+ARG = -1
+WS, FAR = 1 << 50, [(i + 1) << 24 for i in range(12)]
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from rwkvstic_amd import ops as _ops
+    return _ops
+
+
+@pytest.mark.parametrize("T,stride", [(1, 8), (5, 8), (5, 40), (300, 8)])
+@pytest.mark.parametrize("at,size", [("a", 3 * 4 * 16 * 2), ("b", 3 * 8 * 4 * 2), ("adapter", None), ("scale", 3 * 4)])
+def test_adapters_into_what_they_read(T, stride, at, size):
+    from rwkvstic_amd import _native
+    x, a, b, adapter, scale, work = FAR[:6]
+    start = dict(a=a, b=b, adapter=adapter, scale=scale)[at]
+    size = T * 4 if size is None else size
+    rows = ((T - 1) * stride + 8) * 4
+
+    def into(out):
+        return _native.lib().rwkv_lora_rows(None, T, 16, 8, 3, 4, 0, x, 16, 2, a, b, adapter, scale, None, 0, out, stride, work, WS)
+    for out in (start, start + size - 4, start - rows + 4):
+        assert into(out) == ARG, out - start
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 200])
+def test_adapters_beside_what_they_read_and_into_their_rows(ops, T):
+    g = torch.Generator().manual_seed(T)
+    f = lambda *s: torch.randn(*s, generator=g)
+    x, a, b, scale = f(T, 16), f(3, 4, 16), f(3, 16, 4), f(3)
+    adapter = torch.arange(T, dtype=torch.int32) % 4
+    want, bound = P.lora_rows(x, a, b, adapter, scale)
+    near = lambda got: bool(((got.cpu().double() - want).abs() <= 2.0 ** -24 * (bound + want.abs())).all())
+    sizes = [3 * 4 * 16, T * 16, 3 * 16 * 4, T, T * 16, 3]             # a, out, b, adapter, out, scale: one after the other
+    whole = torch.zeros(sum(sizes)).cuda()
+    A, first, B, I, second, S = whole.split(sizes)
+    A.copy_(a.flatten()), B.copy_(b.flatten()), I.view(torch.int32).copy_(adapter), S.copy_(scale)
+    for out in (first, second):
+        assert near(ops.lora_rows(x.cuda(), A.view(3, 4, 16), B.view(3, 16, 4), I.view(torch.int32), S, out=out.view(T, 16)))
+    own = x.cuda()                                    # rows that have been read are free for the result
+    assert near(ops.lora_rows(own, A.view(3, 4, 16), B.view(3, 16, 4), I.view(torch.int32), S, out=own))
+    wide = torch.zeros(T, 48).cuda()
+    wide[:, :16] = x.cuda()
+    assert near(ops.lora_rows(wide[:, :16], A.view(3, 4, 16), B.view(3, 16, 4), I.view(torch.int32), S, out=wide[:, 8:24]))
