@@ -492,7 +492,8 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
  * the K drafts count, cut to 0 .. K; u float32 [B, K+1] in [0, 1).  K <= 64.  A logit that is
  * -infinity or NaN has no weight, +infinity all of it.
  *   tokens int64 [B, K+1]: the accepted drafts, the token drawn, then -1 (in the
- * drawn token's place too, where no logit of the row has weight); accepted int64 [B].
+ * drawn token's place too, where no logit of the row has weight); accepted int64 [B].  Neither shares memory
+ * with the other or with what is read.
  * workspace: rwkv_verify_drafts_workspace_bytes bytes, 16-byte aligned. */
 size_t rwkv_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V);
 int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, int real,

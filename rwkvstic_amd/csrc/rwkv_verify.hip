@@ -441,8 +441,16 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
     RWKV_CHECK_ALIGN(workspace, 16);
     const VerifyPlan pl(B, K, V);
     if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_verify_drafts: workspace too small");
-    uint8_t *ws = (uint8_t *)workspace;
     const bool of_drafts = draft_logits && !greedy && K > 0;
+    const int64_t e = (int64_t)type_bytes(real), token_bytes = B * (K + 1) * 8;
+    auto apart = [&](const void *from, int64_t bytes) {
+        return !from || bytes <= 0 || (!rows_share(1, tokens, 0, token_bytes, from, 0, bytes) && !rows_share(1, accepted, 0, B * 8, from, 0, bytes));
+    };
+    RWKV_CHECK_ARG(apart(logits, ((B - 1) * logits_seq_stride + K * logits_row_stride + V) * e) &&
+                       apart(of_drafts ? draft_logits : nullptr, ((B - 1) * draft_seq_stride + (K - 1) * draft_row_stride + V) * e) && apart(drafts, B * K * 8) &&
+                       apart(lengths, B * 4) && apart(greedy ? nullptr : u, B * (K + 1) * 4) && !rows_share(1, tokens, 0, token_bytes, accepted, 0, B * 8),
+                   "rwkv_verify_drafts: tokens or accepted share memory with another argument");
+    uint8_t *ws = (uint8_t *)workspace;
     const VerifyArgs a{B, K, V, logits, logits_seq_stride, logits_row_stride, of_drafts ? draft_logits : nullptr, draft_seq_stride, draft_row_stride,
                        drafts, lengths, u, 1.0 / std::max(temp, 1e-300), tokens, accepted, pl.segments, pl.segment, (RowStat *)ws, pl.piece, (double *)(ws + pl.stat_bytes),
                        (Verdict *)(ws + pl.stat_bytes + pl.sum_bytes)};

@@ -49,3 +49,24 @@ def test_adapters_beside_what_they_read_and_into_their_rows(ops, T):
     wide = torch.zeros(T, 48).cuda()
     wide[:, :16] = x.cuda()
     assert near(ops.lora_rows(wide[:, :16], A.view(3, 4, 16), B.view(3, 16, 4), I.view(torch.int32), S, out=wide[:, 8:24]))
+
+
+@pytest.mark.parametrize("greedy", [0, 1])
+@pytest.mark.parametrize("which", ["tokens", "accepted"])
+@pytest.mark.parametrize("at", ["logits", "draft", "drafts", "lengths", "u", "other"])
+def test_verdicts_into_what_they_are_made_of(greedy, which, at):
+    """Sequences of logits 1000 apart, their rows 100 apart: to the last logit of the last row."""
+    from rwkvstic_amd import _native
+    B, K, V = 5, 3, 50
+    memory = dict(zip(("logits", "draft", "drafts", "lengths", "u", "tokens", "accepted"), FAR))
+    work = FAR[7]
+    size = {"logits": (4 * 1000 + 3 * 100 + 50) * 8, "draft": (4 * 1000 + 2 * 100 + 50) * 8, "drafts": B * K * 8, "lengths": B * 4, "u": B * (K + 1) * 4,
+            "tokens": B * (K + 1) * 8, "accepted": B * 8}
+    if greedy and at in ("draft", "u"):
+        pytest.skip("not read")
+    other = {"tokens": "accepted", "accepted": "tokens"}[which] if at == "other" else at
+    for to in (memory[other], memory[other] + size[other] - 4, memory[other] - size[which] + 4):
+        m = {**memory, which: to}
+        got = _native.lib().rwkv_verify_drafts(None, B, K, V, 1, m["logits"], 1000, 100, m["draft"], 1000, 100, m["drafts"], m["lengths"], m["u"], 1.0, greedy,
+                                               m["tokens"], m["accepted"], work, WS)
+        assert got == ARG, to - memory[other]
