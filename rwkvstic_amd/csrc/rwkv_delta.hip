@@ -960,7 +960,7 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
     const int64_t o_bytes = T * Hv * dv * e, state_bytes = B * Hv * dk * dv * 4;
     auto apart = [&](const void *from, int64_t bytes) { return !rows_share(1, o, 0, o_bytes, from, 0, bytes) && !rows_share(1, state, 0, state_bytes, from, 0, bytes); };
     RWKV_CHECK_ARG(apart(q, ((T - 1) * q_stride + Hk * dk) * e) && apart(k, ((T - 1) * k_stride + Hk * dk) * e) && apart(v, ((T - 1) * v_stride + Hv * dv) * e) &&
-                       apart(g, T * Hv * 4) && apart(beta, T * Hv * 4) && !rows_share(1, o, 0, o_bytes, state, 0, state_bytes),
+                       apart(g, T * Hv * 4) && apart(beta, T * Hv * 4) && (!starts || apart(starts, (B + 1) * 4)) && !rows_share(1, o, 0, o_bytes, state, 0, state_bytes),
                    "rwkv_delta_rule: o or state shares memory with another argument");
     const DeltaPlan pl(T, B, Hv, dk, dv);
     if (pl.chunks) {

@@ -70,3 +70,35 @@ def test_verdicts_into_what_they_are_made_of(greedy, which, at):
         got = _native.lib().rwkv_verify_drafts(None, B, K, V, 1, m["logits"], 1000, 100, m["draft"], 1000, 100, m["drafts"], m["lengths"], m["u"], 1.0, greedy,
                                                m["tokens"], m["accepted"], work, WS)
         assert got == ARG, to - memory[other]
+
+
+@pytest.mark.parametrize("T", [6, 500])
+@pytest.mark.parametrize("which,size", [("o", 2 * 16 * 4), ("state", 3 * 2 * 16 * 16 * 4)])
+def test_outputs_and_states_into_the_starts(T, which, size):
+    from rwkvstic_amd import _native
+    q, k, v, g, beta, starts, state, o, work = FAR[:9]
+    size *= T if which == "o" else 1
+    for to in (starts, starts + 4 * 4 - 4, starts - size + 4):
+        m = {"state": state, "o": o, which: to}
+        assert _native.lib().rwkv_delta_rule(None, T, 3, 1, 2, 16, 16, 0, q, 16, k, 16, v, 32, g, beta, 1.0, starts, m["state"], m["o"], work, WS) == ARG, to - starts
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [6, 500])
+def test_the_delta_rule_beside_what_it_reads(ops, T):
+    """Everything that is read and written in one buffer, one after the other."""
+    c = P.delta_inputs(T, 3, 1, 2, 16, 16, torch.float32, T)
+    starts = [0, T // 3, T // 2, T]
+    want, after = P.delta_rule(*c, starts, 0.25)
+    s = torch.tensor(starts, dtype=torch.int32)
+    parts = [c[5], s.view(torch.float32), torch.zeros(T, 2, 16), c[0], c[1], c[2], c[3], c[4]]
+    whole = torch.cat([t.flatten() for t in parts]).cuda()
+    at, views = 0, []
+    for t in parts:
+        views.append(whole[at:at + t.numel()].view(t.shape))
+        at += t.numel()
+    state, st, out, q, k, v, g, beta = views
+    ops.delta_rule(q, k, v, g, beta, state, starts=st.view(torch.int32), scale=0.25, out=out)
+    off = 4 * ((T + 64) * (16 + 64)) ** 0.5 * 2.0 ** -24           # rounded sums at random, as elsewhere
+    assert float((out.cpu() - want).abs().max()) <= off * float(want.abs().max()) and float((state.cpu() - after).abs().max()) <= off * float(after.abs().max())
+    assert torch.equal(st.cpu().view(torch.int32), s)
