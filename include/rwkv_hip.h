@@ -443,7 +443,7 @@ typedef enum rwkv_type { RWKV_F32 = 0, RWKV_F64 = 1, RWKV_BF16 = 2, RWKV_F16 = 3
  * out_stride apart; a [N, R, n_in], b [N, n_out, R] of type `low` (RWKV_BF16,
  * RWKV_F16 or RWKV_F32), R <= 256 (adapters of smaller rank are filled with
  * zeros); adapter int32 [T]: a row whose number is not in 0..N-1 has none and
- * gets base[t].  scale float32 [N] or NULL (= 1); base NULL (= 0) or any rows: out
+ * gets base[t], as all do where N is 0 (a and b may be NULL then, R 0).  scale float32 [N] or NULL (= 1); base NULL (= 0) or any rows: out
  * itself, or rows that share no memory with it.  out may lie over x, not over a, b, adapter or scale.
  * What a row holds (infinities, NaN) reaches no other row.
  * workspace: rwkv_lora_rows_workspace_bytes bytes, 16-byte aligned. */

@@ -505,6 +505,7 @@ struct LoraPlan {
         direct = T <= kDirect;
         windows = direct ? 1 : (int)ceil_div(T, kWindow);
         slots = (int)(direct ? T : kWindow / 64 + (N + 1 < kWindow ? N + 1 : kWindow));
+        R = R < 1 ? 1 : R;                                  // (without adapters there may be no rank)
         group = R <= 32 ? 2 : R <= 64 ? 4 : 8;
         groups = (int)ceil_div(R, group * 16);
         ranks = group * groups * 16;
@@ -535,6 +536,7 @@ void launch(hipStream_t st, const LoraPlan &pl, const LoraArgs &p) {
     // 32 rows of lora_down_kernel read the same of a, where that many can be in a tile and their sums stay in registers
     constexpr int kMany = sizeof(Real) == 4 ? 2 : 1;
     auto go_down = [&](auto one, auto many, int group) {
+        if (p.N == 0) return;                 // (every row gets base)
         const int nt = pl.direct ? 1 : kMany;
         const dim3 down((unsigned)(places * (pl.direct ? 1 : 4 / nt) * pl.slices), 1, (unsigned)pl.groups);
         hipLaunchKernelGGL(pl.direct ? one : many, down, dim3(64 * kDownWaves), (size_t)kDownWaves / 2 * nt * group * 64 * 4 * sizeof(Real), st, p);
@@ -564,15 +566,15 @@ using namespace rwkv;
 extern "C" {
 
 size_t rwkv_lora_rows_workspace_bytes(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real) {
-    if (T <= 0 || n_in <= 0 || n_out <= 0 || N <= 0 || R <= 0) return 0;
+    if (T <= 0 || n_in <= 0 || n_out <= 0 || N < 0 || (R <= 0 && N > 0)) return 0;
     return LoraPlan(T, n_in, n_out, N, R, real).bytes();
 }
 
 int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real, const void *x,
                    int64_t x_stride, int low, const void *a, const void *b, const int32_t *adapter, const float *scale, const void *base,
                    int64_t base_stride, void *out, int64_t out_stride, void *workspace, size_t workspace_bytes) {
-    RWKV_CHECK_ARG(x && a && b && adapter && out, "rwkv_lora_rows: null pointer");
-    RWKV_CHECK_ARG(T > 0 && n_in > 0 && n_out > 0 && N > 0 && R > 0, "rwkv_lora_rows: sizes must be positive");
+    RWKV_CHECK_ARG(x && adapter && out && ((a && b) || N == 0), "rwkv_lora_rows: null pointer");
+    RWKV_CHECK_ARG(T > 0 && n_in > 0 && n_out > 0 && N >= 0 && (R > 0 || N == 0), "rwkv_lora_rows: sizes must be positive");
     RWKV_CHECK_ARG(real == RWKV_F32 || real == RWKV_F64, "rwkv_lora_rows: rows are float32 or float64");
     RWKV_CHECK_ARG(low == RWKV_F32 || low == RWKV_BF16 || low == RWKV_F16, "rwkv_lora_rows: adapters are float32, bfloat16 or float16");
     RWKV_CHECK_ARG(x_stride >= 0 && out_stride >= (T > 1 ? n_out : 0) && (!base || base_stride >= 0), "rwkv_lora_rows: row stride too small");

@@ -408,7 +408,8 @@ def lora_rows(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.
 
     ``x [T, n_in]`` and ``base [T, n_out]`` float32 or float64 (products and sums are computed in that type), ``a [N, R, n_in]``
     and ``b [N, n_out, R]`` bfloat16, float16 or float32 with ``R <= 256`` (adapters of smaller rank are filled up with zeros),
-    ``adapter [T]`` int32: a row whose number is outside ``0..N-1`` has no adapter and gets ``base[t]``.  ``scale [N]`` float32;
+    ``adapter [T]`` int32: a row whose number is outside ``0..N-1`` has no adapter and gets ``base[t]``
+    (``N`` may be 0).  ``scale [N]`` float32;
     without it 1.  ``base``: the shared projection's result, without it 0.  ``out`` may be ``base`` itself and may lie
     over ``x``; otherwise it shares no memory with what is read."""
     host = N.host()
