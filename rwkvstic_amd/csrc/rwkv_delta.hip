@@ -963,6 +963,8 @@ int rwkv_delta_rule(rwkv_stream_t stream, int64_t T, int64_t B, int64_t Hk, int6
                        apart(g, T * Hv * 4) && apart(beta, T * Hv * 4) && (!starts || apart(starts, (B + 1) * 4)) && !rows_share(1, o, 0, o_bytes, state, 0, state_bytes),
                    "rwkv_delta_rule: o or state shares memory with another argument");
     const DeltaPlan pl(T, B, Hv, dk, dv);
+    if (pl.chunks ? !launchable(T / kChunk + B, 256) || !launchable(B * Hv * pl.segments * ceil_div(pl.across, 64), kThreads) : !launchable(ceil_div(B * Hv * ceil_div(dv, 16), 4), 256))
+        return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: too many sequences and heads");
     if (pl.chunks) {
         if (q_stride >= (1 << 24) || k_stride >= (1 << 24) || v_stride >= (1 << 24) || Hv * dv >= (1 << 24))
             return set_error(RWKV_ERR_SIZE, "rwkv_delta_rule: rows of 2^24 elements or more");

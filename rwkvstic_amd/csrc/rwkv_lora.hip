@@ -494,6 +494,9 @@ __global__ void __launch_bounds__(256, (Product<Real, Low>::kParts && WIDE && NT
     }
 }
 
+// Tiles of 16 rows to a wavefront of lora_down_kernel where rows are sorted: two read the same of a, where their sums stay in registers.
+constexpr int many_rows(int real) { return real == RWKV_F32 ? 2 : 1; }
+
 // How a call is cut up; the same for its workspace and its launches.
 struct LoraPlan {
     bool direct;
@@ -533,8 +536,7 @@ template <typename Real, typename Low, bool WIDE>
 void launch(hipStream_t st, const LoraPlan &pl, const LoraArgs &p) {
     using Op = Product<Real, Low>;
     const int places = pl.windows * pl.slots;
-    // 32 rows of lora_down_kernel read the same of a, where that many can be in a tile and their sums stay in registers
-    constexpr int kMany = sizeof(Real) == 4 ? 2 : 1;
+    constexpr int kMany = many_rows(sizeof(Real) == 4 ? RWKV_F32 : RWKV_F64);
     auto go_down = [&](auto one, auto many, int group) {
         if (p.N == 0) return;                 // (every row gets base)
         const int nt = pl.direct ? 1 : kMany;
@@ -586,6 +588,9 @@ int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out,
     }
     RWKV_CHECK_ALIGN(workspace, 16);
     const LoraPlan pl(T, n_in, n_out, N, R, real);
+    if (!launchable((int64_t)pl.windows * pl.slots * (pl.direct ? 1 : 4 / many_rows(real)) * pl.slices, 64 * kDownWaves) ||
+        !launchable((int64_t)pl.windows * pl.slots * pl.chunks, 256))
+        return set_error(RWKV_ERR_SIZE, "rwkv_lora_rows: too many rows for so many adapters");
     if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_lora_rows: workspace too small");
     // (x aside: it has been read when the first output is written)
     const int64_t er = (int64_t)type_bytes(real), el = (int64_t)type_bytes(low);

@@ -25,6 +25,9 @@ inline bool rows_share(int64_t T, const void *a, int64_t a_apart, int64_t n, con
     return off < n || off + m > a_apart;
 }
 
+// Whether a launch of this many workgroups has fewer than 2^32 threads, which is what a dispatch counts in 32 bits.
+inline bool launchable(int64_t groups, int64_t threads) { return groups * threads < (1ll << 32); }
+
 // Lets a kernel have this much dynamic LDS where that is over the default limit; asked of the runtime once a device.
 template <auto Kernel> int allow_lds(size_t bytes) {
     if (bytes <= 65536) return RWKV_OK;

@@ -437,7 +437,8 @@ int rwkv_verify_drafts(rwkv_stream_t stream, int64_t B, int64_t K, int64_t V, in
     RWKV_CHECK_ARG(real == RWKV_F32 || real == RWKV_F64, "rwkv_verify_drafts: logits are float32 or float64");
     RWKV_CHECK_ARG(greedy || temp > 0.0, "rwkv_verify_drafts: temp must be positive");
     RWKV_CHECK_ARG(logits_seq_stride >= 0 && logits_row_stride >= 0 && draft_seq_stride >= 0 && draft_row_stride >= 0, "rwkv_verify_drafts: negative stride");
-    if (K > kMaxDrafts || V >= (1ll << 31) || B >= (1ll << 24)) return set_error(RWKV_ERR_SIZE, "rwkv_verify_drafts: at most %d drafts", kMaxDrafts);
+    if (K > kMaxDrafts || V >= (1ll << 31)) return set_error(RWKV_ERR_SIZE, "rwkv_verify_drafts: at most %d drafts", kMaxDrafts);
+    if (B >= (1ll << 24) || !launchable(B * (2 * K + 1), kVT) || !launchable(B, kDT)) return set_error(RWKV_ERR_SIZE, "rwkv_verify_drafts: too many sequences");
     RWKV_CHECK_ALIGN(workspace, 16);
     const VerifyPlan pl(B, K, V);
     if (!workspace || workspace_bytes < pl.bytes()) return set_error(RWKV_ERR_WORKSPACE, "rwkv_verify_drafts: workspace too small");

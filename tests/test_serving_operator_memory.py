@@ -102,3 +102,24 @@ def test_the_delta_rule_beside_what_it_reads(ops, T):
     off = 4 * ((T + 64) * (16 + 64)) ** 0.5 * 2.0 ** -24           # rounded sums at random, as elsewhere
     assert float((out.cpu() - want).abs().max()) <= off * float(want.abs().max()) and float((state.cpu() - after).abs().max()) <= off * float(after.abs().max())
     assert torch.equal(st.cpu().view(torch.int32), s)
+
+
+def test_more_than_a_launch_can_take():
+    """Refused for their size before the workspace is looked at; nothing is launched."""
+    from rwkvstic_amd import _native
+    L = _native.lib()
+    SIZE, WORKSPACE = -3, -4
+    far = [(i + 1) << 50 for i in range(10)]
+
+    def lora(T, N, real=0):
+        return L.rwkv_lora_rows(None, T, 16, 8, N, 4, real, far[0], 16, 2, far[1], far[2], far[3], None, None, 0, far[4], 8, far[5], 0)
+    assert lora(1 << 24, 1) == WORKSPACE and lora(1 << 22, 500) == WORKSPACE and lora(1 << 22, 1024) == SIZE and lora(1 << 21, 1024, 1) == SIZE
+
+    def delta(B, T=None, Hv=64):
+        T = B if T is None else T
+        return L.rwkv_delta_rule(None, T, B, 1, Hv, 4, 4, 0, far[0], 4, far[1], 4, far[2], 4 * Hv, far[3], far[4], 1.0, far[5], far[6], far[7], far[8], 0)
+    assert delta(1 << 20) == SIZE and delta(1 << 20, 50 << 20, 1) == WORKSPACE and delta(1 << 24, 50 << 24, 1) == SIZE
+
+    def verify(B, K):
+        return L.rwkv_verify_drafts(None, B, K, 4, 0, far[0], 4 * (K + 1), 4, far[1], 4 * K, 4, far[2], None, far[3], 1.0, 0, far[4], far[5], far[6], 0)
+    assert verify(1 << 21, 0) == WORKSPACE and verify(1 << 22, 0) == SIZE and verify(1 << 17, 63) == WORKSPACE and verify(1 << 18, 63) == SIZE
