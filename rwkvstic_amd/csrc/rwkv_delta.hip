@@ -13,9 +13,10 @@
 // and the segments are gone through once more from there, for their outputs.
 // Both on the matrix cores with float32 sums; G and its differences are float64, as a decay is the exponential of a difference of sums.
 // A float32 operand goes into the bfloat16 matrix instructions as the sum of three bfloat16 values, its 24 bits cut in three
-// (planes); of the products of planes those below 2^-24 are left out: three products with bfloat16 keys, six of two float32
-// operands, against 16 times the time of one for float32 instructions.  (Two planes for what only reaches a bfloat16 output are not
-// enough: with keys that repeat, Q S and P U cancel.)
+// (planes); of the products of planes those whose numbers (0, 1, 2) add up to three or more are left out, 2^-24.5 of a product
+// on average, 2^-21 at most: three products with bfloat16 keys (nothing left out), six of two float32 operands, against 16 times the
+// time of one for float32 instructions.  (Two planes for what only reaches a bfloat16 output are not enough: with keys that repeat,
+// Q S and P U cancel.)
 #include "rwkv_types.h"
 
 #include <type_traits>
@@ -365,8 +366,10 @@ __global__ void __launch_bounds__(256) delta_within_kernel(DeltaArgs a, f32x4 *s
         for (int r = 0; r < 16; ++r) s_X[wave][r][lane] = x[r];
     }
     __syncthreads();
-    // ... the others below them, a wavefront to a column of blocks: X_mc = -X_mm sum_l A_ml X_lc; 0 above the diagonal.  Without
-    // branches: behind one on the wavefront's number the compiler left out the wait (10 instructions) that reading a product's registers needs.
+    // ... the others below them, a wavefront to a column of blocks: X_mc = -X_mm sum_l A_ml X_lc; 0 above the diagonal.  Chosen without
+    // branches: with "if (m > wave)" around the products, wave being scalar, what clang 22 builds goes from a product through two jumps
+    // to the read of its registers, 3 instructions where 10 are needed, and T came out wrong.  (With a wave that differs from lane to lane
+    // it waits, and so it does where the branches of products() above meet.)
     f32x4 X[4];
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -863,6 +866,8 @@ __global__ void __launch_bounds__(kThreads) delta_chunks_f32_kernel(DeltaArgs a,
 
 // Chunks from this many rows a sequence on.  (32 heads of 128 x 128, bfloat16, 16 sequences of 32 rows: 86 us in chunks, 72 in steps; of
 // 48: 93 and 95; of 64: 101 and 125.  64 sequences: 310 and 227, 366 and 325, 451 and 429; one: 24 and 28, 25 and 39, 26 and 51.)
+// It is the average that counts, as the host does not know the lengths: a long sequence among many short ones, fewer rows than this on
+// average, goes step by step too (2000 rows among 63 single ones: 1490 us, where alone they take 152 in chunks).
 constexpr int kManyRows = 48;
 bool in_chunks(int64_t T, int64_t B) { return T >= kManyRows * B; }
 

@@ -9,8 +9,8 @@
 //   lora_down_kernel   a wavefront per 16 rows, up to 128 ranks and slice of n_in: parts of h
 //   lora_up_kernel     a workgroup per tile and range of n_out: the parts added up into LDS, then b h on top of base
 // Memory bounds them where rows or adapters are many: 2048 rows, 5120 to 20480, 8 bfloat16 adapters of rank 128, float32 rows: 6 + 39 +
-// 118 us, the last one at 3.2 TB/s.  Float64 rows, 1024 of 2560 to 2560, 5 adapters of rank 32: 5 + 14 + 15 us (matrix instructions of 64
-// clocks, and 21 MB each way).  One row: 4 + 4 us, each the time from an empty kernel's start to its first loads and back.
+// 118 us, the last one at 3.2 TB/s.  Float64 rows, 1024 of 2560 to 2560, 5 adapters of rank 32: 5 + 13 + 15 us (5 of them
+// matrix instructions; the rest is few workgroups that wait twice for their own loads, and 21 MB each way).  One row: 4 + 4 us, each the time from an empty kernel's start to its first loads and back.
 #include "rwkv_types.h"
 
 namespace rwkv {

@@ -6,7 +6,7 @@
 //   verify_left_kernel  which drafts are accepted, and the sums of what the next token is drawn from, piece by piece
 //   verify_pick_kernel  the piece that the drawn token is in, and the token
 // Of the logits the first kernel reads everything once; the others read one row of each a sequence (from cache).  64 sequences of
-// 8 drafts, 65536 tokens, float32, with the drafts' logits: 63 us (4.5 TB/s) + 20 + 7; one of 4, 50277 tokens, float64: 5 + 6 + 6, latency.
+// 8 drafts, 65536 tokens, float32, with the drafts' logits: 64 us (4.5 TB/s) + 21 + 7; one of 4, 50277 tokens, float64: 5 + 6 + 6, latency.
 #include "rwkv_types.h"
 
 #include <algorithm>

@@ -455,7 +455,9 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     ``state [B, Hv, dk, dv]`` float32, updated in place.  ``starts [B + 1]`` int32 on the device: sequence ``b`` is the rows
     ``starts[b]`` to ``starts[b + 1] - 1``; without it ``T / B`` rows each.  ``scale``: ``dk ** -0.5`` unless given.
     Returns ``o [T, Hv, dv]`` of v's type (``out``, which shares no memory with the arguments); rows of no sequence are not written,
-    and an empty sequence keeps its state."""
+    and an empty sequence keeps its state.  From 48 rows a sequence on, on average, chunks of 64 rows are computed at once: a value in them
+    that is not finite reaches rows of the chunk before it too, though no other sequence, and keys with ``beta k.k`` over 2 may overflow
+    where single steps do not."""
     scale = None if scale is None else float(scale)
     host = N.host()
     y = host and host.delta_rule(q, k, v, g, beta, state, starts, scale if scale is not None else _default_scale(q), out)
@@ -500,7 +502,8 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: Optional[torch.
     first refused one a token is drawn from ``max(p - q, 0)``, after the last from ``p``, by ``u[b, K]`` (``u [B, K+1]`` float32 in [0, 1)):
     the lowest index at which the running weight exceeds ``u`` times the whole.  ``draft_logits [B, K, V]`` of logits' type; without them
     the drafts have no distribution of their own (``q(d) = 1``).  ``greedy``: a draft is accepted while it is the first maximum, and the
-    token drawn is that maximum.  Row ``b`` of ``tokens`` is the accepted drafts, the token drawn, then -1 (there too, where no logit has weight)."""
+    token drawn is that maximum.  Logits of -infinity are left out: a sampler that keeps only some of the tokens (``sample_token`` does, as
+    ``typical``) is verified against once the others are set to that.  Row ``b`` of ``tokens`` is the accepted drafts, the token drawn, then -1 (there too, where no logit has weight)."""
     temp, greedy = float(temp), bool(greedy)
     host = N.host()
     y = host and host.verify_drafts(logits, drafts, u, draft_logits, lengths, temp, greedy)
