@@ -445,7 +445,8 @@ typedef enum rwkv_type { RWKV_F32 = 0, RWKV_F64 = 1, RWKV_BF16 = 2, RWKV_F16 = 3
  * zeros); adapter int32 [T]: a row whose number is not in 0..N-1 has none and
  * gets base[t], as all do where N is 0 (a and b may be NULL then, R 0).  scale float32 [N] or NULL (= 1); base NULL (= 0) or any rows: out
  * itself, or rows that share no memory with it.  out may lie over x, not over a, b, adapter or scale.
- * What a row holds (infinities, NaN) reaches no other row.
+ * What a row holds (infinities, NaN) reaches no other row.  With float32 rows and
+ * bfloat16 adapters a value under 2^-103 counts to 2^-125 only.
  * workspace: rwkv_lora_rows_workspace_bytes bytes, 16-byte aligned. */
 size_t rwkv_lora_rows_workspace_bytes(int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R, int real);
 int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out, int64_t N, int64_t R,
@@ -468,7 +469,8 @@ int rwkv_lora_rows(rwkv_stream_t stream, int64_t T, int64_t n_in, int64_t n_out,
  * of an empty sequence is.  Long sequences are computed in chunks of 64 rows, in which
  * a value that is not finite reaches rows before it too, but no other sequence; keys
  * with beta k.k over 2 make the state grow from row to row, and what it would be without
- * values may then overflow where the state itself does not.  o and state share no memory
+ * values may then overflow where the state itself does not; values under 2^-103 count
+ * to 2^-125 only.  o and state share no memory
  * with each other or with what is read.  dk <= 256, and in chunks (48 rows a sequence and
  * more) rows and strides below 2^24 elements.  workspace: rwkv_delta_rule_workspace_bytes bytes, 16-byte aligned. */
 size_t rwkv_delta_rule_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t dk, int64_t dv);

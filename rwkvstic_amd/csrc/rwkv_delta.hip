@@ -14,7 +14,7 @@
 // Both on the matrix cores with float32 sums; G and its differences are float64, as a decay is the exponential of a difference of sums.
 // A float32 operand goes into the bfloat16 matrix instructions as the sum of three bfloat16 values, its 24 bits cut in three
 // (planes); of the products of planes those whose numbers (0, 1, 2) add up to three or more are left out, 2^-24.5 of a product
-// on average, 2^-21 at most: three products with bfloat16 keys (nothing left out), six of two float32 operands, against 16 times the
+// on average, 2^-21 at most (and planes under 2^-126, which the instructions take for 0: up to 2^-125 of a value under 2^-103): three products with bfloat16 keys (nothing left out), six of two float32 operands, against 16 times the
 // time of one for float32 instructions.  (Two planes for what only reaches a bfloat16 output are not enough: with keys that repeat,
 // Q S and P U cancel.)
 #include "rwkv_types.h"

@@ -105,7 +105,9 @@ template <typename Real, typename Low> struct Product {
 };
 
 // float32 rows and bfloat16 adapters: a float32 value is the sum of three bfloat16 ones, its 24 bits cut in three, so that three
-// bfloat16 products with float32 sums lose nothing, in a fifth of the matrix cores' time for float32 operands.  But for infinities:
+// bfloat16 products with float32 sums lose nothing, in a fifth of the matrix cores' time for float32 operands.  But for parts under
+// 2^-126, which the instructions take for 0: of a value under 2^-103 up to 2^-125 can be lost (float32 instructions lose
+// none), which does not show beside terms of ordinary size.  And but for infinities:
 // one has no rest, and a part that is 0 must not meet one.  A sum with an infinite term comes out as no number, or right; the sums that
 // are none are taken again of whole operands (kParts), so that they are what the other types' are.
 template <> struct Product<float, __bf16> {
